@@ -162,6 +162,139 @@ TIMESTRAL_API int tsb_refine_static(const float* d_q, const float* d_rows, const
                                     int32_t patches, int32_t patch_size, int32_t num_quantiles, int32_t median_index,
                                     double minimum_scale, float* d_out, void* stream);
 
+/* ---- attention over a paged cache -----------------------------------------------------
+ * No counterpart in the reference, which runs every decode block over its whole context
+ * (src/forecaster.cpp:19-67). Three operators on caller device buffers for programs that
+ * decode step by step and keep the keys and values of earlier tokens: the per-head RMS norm
+ * and rotation of queries and keys, writing keys and values into a paged cache, and
+ * attention of new tokens over that cache.
+ *
+ * Common rules. Every pointer is memory of the current device (anything else is refused with
+ * TSB_ERR_ARG), as is `stream` (cudaStream_t, NULL = legacy default stream). Calls enqueue
+ * work and return; they allocate nothing, keep nothing between calls and may be captured into
+ * a CUDA graph. Values are f16 or bf16, sums and statistics f32, each result is rounded once.
+ * The last axis (head_dim) is contiguous; every data pointer is 16-byte aligned and every
+ * stride, in elements, a multiple of 8. Offsets are 64-bit. Argument errors go to
+ * timestral_capi_last_error(NULL).
+ *
+ * What only the device can see (positions, page numbers, lengths) is checked there: `error`
+ * (a device int32, or NULL) receives the code of the first such fault found, and is left
+ * alone otherwise, so a caller clears it once and reads it when it likes. */
+enum { TSB_TYPE_F16 = 1, TSB_TYPE_BF16 = 30 };   /* GGUF type numbers */
+enum {
+    TSB_FAULT_WAIT = 5,      /* a bounded wait expired: the call's results are incomplete */
+    TSB_FAULT_POSITION = 6,  /* a position outside the rotation table: that token is not written */
+    TSB_FAULT_BATCH = 10,    /* q_start or lengths contradict each other or the given bounds: that
+                                sequence is skipped, its rows left as they were */
+    TSB_FAULT_PAGE = 11,     /* a page number outside the pool: nothing is written there, and its
+                                keys and values read as zeros */
+};
+
+/* [tokens][heads][head_dim]: element (t, h, d) at data[t * token_stride + h * head_stride + d]. */
+typedef struct tsb_heads {
+    void* data;
+    int64_t token_stride, head_stride;
+} tsb_heads;
+
+/* A cache in pages. Position p of sequence s lies in page table[s * table_stride + p / page_size],
+ * slot p % page_size; element (page, head, slot, d) at k[page * page_stride + head * head_stride +
+ * slot * slot_stride + d], and so for v. page_size is a power of two from 8 to 1024, head_dim 64
+ * or 128. Table entries of pages that no visible position lies in are never read as pages. */
+typedef struct tsb_paged_cache {
+    void* k;
+    void* v;
+    int64_t k_page_stride, k_head_stride, k_slot_stride;
+    int64_t v_page_stride, v_head_stride, v_slot_stride;
+    const int32_t* table;
+    int64_t table_stride;
+    int32_t table_width;     /* entries of one sequence */
+    int32_t type, num_pages, page_size, kv_heads, head_dim;
+} tsb_paged_cache;
+
+/* The new tokens of each sequence: tokens q_start[s] .. q_start[s + 1] - 1 of the token arrays,
+ * the last q_start[s + 1] - q_start[s] of its lengths[s] positions (lengths count the new
+ * tokens). A sequence may have no new token. max_chunk and max_length bound the new tokens
+ * and the length of every sequence; a captured graph serves any batch within them. Token rows
+ * outside every sequence are left as they were. */
+typedef struct tsb_paged_batch {
+    const int32_t* q_start;  /* [seqs + 1] */
+    const int32_t* lengths;  /* [seqs] */
+    int32_t seqs, max_chunk, max_length;
+} tsb_paged_batch;
+
+/* Rotation of the first rope_dim values of a head (a multiple of 16): value d and value
+ * d + rope_dim / 2 turn by the angle whose cosine and sine stand at
+ * cos/sin[position * stride + d], d < rope_dim / 2. cos == NULL: no rotation. */
+typedef struct tsb_rotation {
+    const float* cos;
+    const float* sin;
+    int64_t stride;          /* floats between positions: a multiple of 4 (tables 16-byte aligned) */
+    int32_t rows;            /* positions in the tables */
+    int32_t rope_dim;
+    const int32_t* positions;  /* [tokens]; NULL (tsb_paged_append): the position in the cache */
+} tsb_rotation;
+
+/* x * 1/sqrt(mean(x^2) + eps) * weight over each head (weight [head_dim] f32; NULL: no norm),
+ * then the rotation, of `tokens` tokens' q_heads queries and k_heads keys (k_heads 0: queries
+ * alone). head_dim: a multiple of 16 up to 256. Outputs may be the inputs themselves (same
+ * pointer and strides); otherwise they must not overlap them. */
+typedef struct tsb_norm_rope_args {
+    int32_t type, tokens, head_dim, q_heads, k_heads;
+    float eps;
+    tsb_heads q, q_out, k, k_out;
+    const float* q_weight;
+    const float* k_weight;
+    tsb_rotation rotation;
+    int32_t* error;
+} tsb_norm_rope_args;
+TIMESTRAL_API int tsb_norm_rope(const tsb_norm_rope_args* args, void* stream);
+
+/* Write the keys and values of the new tokens (k, v: `tokens` rows of the cache's kv_heads) at
+ * their positions of the cache, the keys normed with k_weight (as tsb_norm_rope; NULL: not)
+ * and rotated on the way. Two sequences that share a page (a common prefix) must not write the
+ * same position. */
+typedef struct tsb_paged_append_args {
+    const tsb_paged_cache* cache;
+    const tsb_paged_batch* batch;
+    tsb_heads k, v;
+    int32_t tokens;
+    float eps;
+    const float* k_weight;
+    tsb_rotation rotation;
+    int32_t* error;
+} tsb_paged_append_args;
+TIMESTRAL_API int tsb_paged_append(const tsb_paged_append_args* args, void* stream);
+
+/* out = gate * softmax(scale * q . k) v of every new token over the cache, which holds the new
+ * tokens' own keys and values already. q_heads is a multiple of the cache's kv_heads; query head
+ * h reads cached head h / (q_heads / kv_heads). The token at position p sees the positions j <= p,
+ * with window > 0 those with j > p - window, and with key_valid those whose bit is set (bit j % 32
+ * of word j / 32 of the sequence's row; positions from key_valid_positions on count as set),
+ * self_visible adding j = p whatever its bit. A token that sees nothing gives zeros. What stands in
+ * the cache at positions that no token of the sequence sees (NaN too) does not reach the results.
+ * gate (as q) may be NULL; out may be q itself. scale 0 means 1 / sqrt(head_dim).
+ * The keys of few rows are split between blocks, as far as `workspace` holds their partial
+ * results; tsb_paged_attention_workspace gives the bytes that the call can use at most (NULL and 0
+ * are allowed). A workspace serves one call at a time: calls that may overlap on the GPU (other
+ * streams, two graphs) need one each. Results do not depend on what it held. */
+typedef struct tsb_paged_attention_args {
+    const tsb_paged_cache* cache;
+    const tsb_paged_batch* batch;
+    tsb_heads q, out, gate;
+    int32_t tokens, q_heads, window, self_visible;
+    float scale;
+    int32_t key_valid_positions;
+    const int32_t* key_valid;
+    int64_t key_valid_stride;   /* words of one sequence */
+    void* workspace;
+    size_t workspace_bytes;
+    int32_t* error;
+} tsb_paged_attention_args;
+TIMESTRAL_API int tsb_paged_attention(const tsb_paged_attention_args* args, void* stream);
+/* Bytes of workspace that lets a call with these arguments split as it would like to (0: it
+ * does not split). Only cache, batch (bounds), tokens, q_heads and window are read. */
+TIMESTRAL_API size_t tsb_paged_attention_workspace(const tsb_paged_attention_args* args);
+
 /* ---- kernel-level test entries (device pointers) ---------------------------------- */
 typedef struct tsb_gemm_test {
     int32_t kind;                 /* 0 f32, 1 f16, 2 resid, 3 silu, 4 swiglu, 5 vgate, 6 qkvg */

@@ -64,6 +64,8 @@ enum DeviceError : int {
     kDevNaN = 7,              // a capped forecast value is NaN (reference: degenerate input)
     kDevNonFinite = 8,        // a final forecast value is not finite
     kDevTimeoutConv = 9,      // Q8_0 GEMM: weights never converted / int8 stage never filled
+    kDevBadBatch = 10,        // paged cache: q_start or lengths outside the given bounds
+    kDevBadPage = 11,         // paged cache: a page number outside the pool
 };
 
 __device__ __forceinline__ void record_error(int* err, int code) {

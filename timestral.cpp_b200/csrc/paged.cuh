@@ -1,0 +1,149 @@
+// Operators over a paged cache of keys and values (include/timestral_b200.h): what their
+// kernels share. The host entries (paged_api.cu) check the arguments and fill these structs.
+#pragma once
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "common.cuh"
+
+namespace tsb {
+
+// [tokens][heads][head_dim], strides in elements.
+struct PagedHeads {
+    void* data = nullptr;
+    int64_t token = 0, head = 0;
+};
+
+struct PagedRotation {
+    const float* cos = nullptr;
+    const float* sin = nullptr;
+    int64_t stride = 0;
+    int rows = 0, dim = 0;
+    const int* positions = nullptr;
+};
+
+struct PagedCache {
+    void* k = nullptr;
+    void* v = nullptr;
+    int64_t k_page = 0, k_head = 0, k_slot = 0, v_page = 0, v_head = 0, v_slot = 0;
+    const int* table = nullptr;
+    int64_t table_stride = 0;
+    int num_pages = 0, page_shift = 0, kv_heads = 0, head_dim = 0;
+};
+
+struct PagedBatch {
+    const int* q_start = nullptr;
+    const int* lengths = nullptr;
+    int seqs = 0, max_chunk = 0, max_length = 0, tokens = 0;
+};
+
+struct NormRopeSide {
+    PagedHeads in, out;
+    const float* weight = nullptr;
+    int heads = 0;
+};
+struct NormRope {
+    NormRopeSide q, k;
+    PagedRotation rot;
+    int tokens = 0, head_dim = 0;
+    float eps = 0;
+    int* err = nullptr;
+};
+
+struct PagedAppend {
+    PagedCache cache;
+    PagedBatch batch;
+    PagedHeads k, v;
+    const float* k_weight = nullptr;
+    PagedRotation rot;
+    float eps = 0;
+    int* err = nullptr;
+};
+
+struct PagedAttention {
+    PagedCache cache;
+    PagedBatch batch;
+    PagedHeads q, out, gate;
+    int q_heads = 0, group = 0, window = 0, self_visible = 0;
+    float scale_log2 = 0;               // scale * log2(e)
+    const uint32_t* key_valid = nullptr;
+    int64_t key_valid_stride = 0;
+    int key_valid_positions = 0;
+    int splits = 1;
+    float* part_o = nullptr;            // [splits][tokens * q_heads][head_dim], unnormalised
+    float2* part_ml = nullptr;          // [splits][tokens * q_heads]: reference maximum (log2 units), sum
+    int* err = nullptr;
+};
+
+// How a call of paged_attention runs: chosen from sizes alone, so that the workspace query and
+// the call agree. splits is what it would like without a bound on the workspace.
+struct PagedPlan {
+    int splits = 1;
+    size_t split_bytes = 0;             // workspace bytes of one split
+};
+PagedPlan paged_plan(const PagedAttention& a);
+
+// bf16: values of type bf16, else f16.
+cudaError_t norm_rope(const NormRope& a, bool bf16, cudaStream_t stream);
+cudaError_t paged_append(const PagedAppend& a, bool bf16, cudaStream_t stream);
+cudaError_t paged_attention(const PagedAttention& a, bool bf16, cudaStream_t stream);
+
+// ---------------------------------------------------------------------------------------
+// Device helpers
+
+// The new tokens of sequence s, checked against the bounds the host gave; a contradiction is
+// recorded and gives ok = false.
+struct SeqInfo { int start, n, len; bool ok; };
+__device__ __forceinline__ SeqInfo load_seq(const PagedBatch& b, int s, int* err) {
+    SeqInfo q;
+    q.start = b.q_start[s];
+    const int end = b.q_start[s + 1];
+    q.len = b.lengths[s];
+    // compared before they are subtracted: any two ints may stand there
+    q.ok = q.start >= 0 && end >= q.start && end <= b.tokens && q.len >= 0 && q.len <= b.max_length &&
+           end - q.start <= b.max_chunk && end - q.start <= q.len;
+    q.n = q.ok ? end - q.start : 0;
+    if (!q.ok) record_error(err, kDevBadBatch);
+    return q;
+}
+
+template <class T>
+struct Pair;
+template <>
+struct Pair<__half> {
+    static __device__ __forceinline__ float2 up(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
+    static __device__ __forceinline__ uint32_t down(float a, float b) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+};
+template <>
+struct Pair<__nv_bfloat16> {
+    static __device__ __forceinline__ float2 up(uint32_t u) {
+        return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+    }
+    static __device__ __forceinline__ uint32_t down(float a, float b) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+};
+// Eight 16-bit values <-> floats.
+template <class T>
+__device__ __forceinline__ void unpack8(const uint4& u, float (&f)[8]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 p = Pair<T>::up(w[i]);
+        f[2 * i] = p.x;
+        f[2 * i + 1] = p.y;
+    }
+}
+template <class T>
+__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+    return make_uint4(Pair<T>::down(f[0], f[1]), Pair<T>::down(f[2], f[3]), Pair<T>::down(f[4], f[5]),
+                      Pair<T>::down(f[6], f[7]));
+}
+
+}  // namespace tsb

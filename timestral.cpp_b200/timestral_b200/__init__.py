@@ -39,6 +39,56 @@ class GemmTest(C.Structure):
                 ("Bs", C.c_void_p), ("lds", C.c_int64)]
 
 
+class Heads(C.Structure):
+    """tsb_heads (include/timestral_b200.h), strides in elements."""
+    _fields_ = [("data", C.c_void_p), ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class PagedCacheArgs(C.Structure):
+    """tsb_paged_cache."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_page_stride", C.c_int64), ("k_head_stride", C.c_int64),
+                ("k_slot_stride", C.c_int64), ("v_page_stride", C.c_int64), ("v_head_stride", C.c_int64),
+                ("v_slot_stride", C.c_int64), ("table", C.c_void_p), ("table_stride", C.c_int64),
+                ("table_width", C.c_int32), ("type", C.c_int32), ("num_pages", C.c_int32),
+                ("page_size", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32)]
+
+
+class PagedBatchArgs(C.Structure):
+    """tsb_paged_batch."""
+    _fields_ = [("q_start", C.c_void_p), ("lengths", C.c_void_p), ("seqs", C.c_int32), ("max_chunk", C.c_int32),
+                ("max_length", C.c_int32)]
+
+
+class Rotation(C.Structure):
+    """tsb_rotation."""
+    _fields_ = [("cos", C.c_void_p), ("sin", C.c_void_p), ("stride", C.c_int64), ("rows", C.c_int32),
+                ("rope_dim", C.c_int32), ("positions", C.c_void_p)]
+
+
+class NormRopeArgs(C.Structure):
+    """tsb_norm_rope_args."""
+    _fields_ = [("type", C.c_int32), ("tokens", C.c_int32), ("head_dim", C.c_int32), ("q_heads", C.c_int32),
+                ("k_heads", C.c_int32), ("eps", C.c_float), ("q", Heads), ("q_out", Heads), ("k", Heads),
+                ("k_out", Heads), ("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("rotation", Rotation),
+                ("error", C.c_void_p)]
+
+
+class PagedAppendArgs(C.Structure):
+    """tsb_paged_append_args."""
+    _fields_ = [("cache", C.POINTER(PagedCacheArgs)), ("batch", C.POINTER(PagedBatchArgs)), ("k", Heads), ("v", Heads),
+                ("tokens", C.c_int32), ("eps", C.c_float), ("k_weight", C.c_void_p), ("rotation", Rotation),
+                ("error", C.c_void_p)]
+
+
+class PagedAttentionArgs(C.Structure):
+    """tsb_paged_attention_args."""
+    _fields_ = [("cache", C.POINTER(PagedCacheArgs)), ("batch", C.POINTER(PagedBatchArgs)), ("q", Heads), ("out", Heads),
+                ("gate", Heads), ("tokens", C.c_int32), ("q_heads", C.c_int32), ("window", C.c_int32),
+                ("self_visible", C.c_int32), ("scale", C.c_float), ("key_valid_positions", C.c_int32),
+                ("key_valid", C.c_void_p), ("key_valid_stride", C.c_int64), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t), ("error", C.c_void_p)]
+
+
 _lib = None
 
 # Every symbol the headers in include/ declare, with (restype, argtypes).
@@ -87,6 +137,10 @@ SIGNATURES = {
     "tsb_test_fail_workspace_allocations": (C.c_int, [C.c_int32]),
     "tsb_test_device_reset": (C.c_int, []),
     "tsb_refine_static": (C.c_int, [C.c_void_p] * 6 + [C.c_int32] * 6 + [C.c_double, C.c_void_p, C.c_void_p]),
+    "tsb_norm_rope": (C.c_int, [C.POINTER(NormRopeArgs), C.c_void_p]),
+    "tsb_paged_append": (C.c_int, [C.POINTER(PagedAppendArgs), C.c_void_p]),
+    "tsb_paged_attention": (C.c_int, [C.POINTER(PagedAttentionArgs), C.c_void_p]),
+    "tsb_paged_attention_workspace": (C.c_size_t, [C.POINTER(PagedAttentionArgs)]),
 }
 
 
@@ -258,3 +312,6 @@ class Model:
     @property
     def tensor_core_path(self) -> bool:
         return lib().tsb_model_path(self.h) == 1
+
+
+from .paged import PagedBatch, PagedCache, norm_rope, paged_append, paged_attention, paged_attention_workspace  # noqa: E402,F401

@@ -887,6 +887,21 @@ bool make_map_3d_f16(CUtensorMap* map, const void* base, int64_t planes, int64_t
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// 4D map of 16-bit values over {width values, three outer axes with their sizes and strides in
+// elements (ascending)}; box {64 values, box[0], box[1], box[2]}, 128-byte swizzle, zeros outside.
+bool make_map_4d_16bit(CUtensorMap* map, const void* base, bool bf16, int width, const int64_t (&size)[3],
+                       const int64_t (&stride)[3], const int (&box_rows)[3]) {
+    auto fn = encode_fn();
+    if (!fn) return false;
+    cuuint64_t dims[4] = {cuuint64_t(width), cuuint64_t(size[0]), cuuint64_t(size[1]), cuuint64_t(size[2])};
+    cuuint64_t strides[3] = {cuuint64_t(stride[0]) * 2, cuuint64_t(stride[1]) * 2, cuuint64_t(stride[2]) * 2};
+    cuuint32_t box[4] = {64, cuuint32_t(box_rows[0]), cuuint32_t(box_rows[1]), cuuint32_t(box_rows[2])};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base),
+              dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // 3D f16 tensor map over head-major [rows][slots][64] (slots = heads x tokens of a row), box
 // {64, 1 slot, box_rows rows}: the same (head, token) slot of box_rows consecutive rows, laid
 // out in shared memory as box_rows 128-byte rows (the image of a 2D box of box_rows rows).

@@ -80,6 +80,7 @@ struct PagedAttention {
 // How a call of paged_attention runs: chosen from sizes alone, so that the workspace query and
 // the call agree. splits is what it would like without a bound on the workspace.
 struct PagedPlan {
+    bool tiles = false;                 // paged_attention_tiles, else paged_attention_rows
     int splits = 1;
     size_t split_bytes = 0;             // workspace bytes of one split
 };
@@ -89,6 +90,10 @@ PagedPlan paged_plan(const PagedAttention& a);
 cudaError_t norm_rope(const NormRope& a, bool bf16, cudaStream_t stream);
 cudaError_t paged_append(const PagedAppend& a, bool bf16, cudaStream_t stream);
 cudaError_t paged_attention(const PagedAttention& a, bool bf16, cudaStream_t stream);
+// The kernel for many rows (paged_tiles.cu): *taken is false, and nothing was launched, when the
+// cache's strides do not fit a tensor map.
+cudaError_t paged_attention_tiles(const PagedAttention& a, bool bf16, cudaStream_t stream, bool* taken);
+constexpr int kPagedTileRows = 256;     // its rows per block
 
 // ---------------------------------------------------------------------------------------
 // Device helpers
@@ -144,6 +149,17 @@ template <class T>
 __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
     return make_uint4(Pair<T>::down(f[0], f[1]), Pair<T>::down(f[2], f[3]), Pair<T>::down(f[4], f[5]),
                       Pair<T>::down(f[6], f[7]));
+}
+
+// Keys [k0, k0 + 64) of the sequence whose bits are set (all of them without key_valid).
+__device__ __forceinline__ uint64_t valid_bits(const PagedAttention& a, int seq, int k0) {
+    if (!a.key_valid || k0 >= a.key_valid_positions) return ~0ull;
+    const uint32_t* w = a.key_valid + int64_t(seq) * a.key_valid_stride + (k0 >> 5);
+    const int left = a.key_valid_positions - k0;
+    uint64_t m = w[0];
+    if (left > 32) m |= uint64_t(w[1]) << 32;
+    if (left < 64) m |= ~0ull << left;
+    return m;
 }
 
 }  // namespace tsb

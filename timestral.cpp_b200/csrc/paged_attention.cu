@@ -16,12 +16,6 @@ int device_sm_count();
 
 namespace {
 
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // ---------------------------------------------------------------------------------------
 // Few rows (single tokens, short chunks): 16 * RG rows a block on mma.sync, bound by the bytes of
 // the cache. Four warps: RG row groups of 16 rows, 4 / RG key groups that share each 64-key tile
@@ -63,17 +57,6 @@ __device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
 // 16 bytes, or zeros without reading `src`.
 __device__ __forceinline__ void cp_async16_if(uint32_t dst, const void* src, bool read) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(read ? 16 : 0) : "memory");
-}
-
-// Keys [k0, k0 + 64) of the sequence whose bits are set (all of them without key_valid).
-__device__ __forceinline__ uint64_t valid_bits(const PagedAttention& a, int seq, int k0) {
-    if (!a.key_valid || k0 >= a.key_valid_positions) return ~0ull;
-    const uint32_t* w = a.key_valid + int64_t(seq) * a.key_valid_stride + (k0 >> 5);
-    const int left = a.key_valid_positions - k0;
-    uint64_t m = w[0];
-    if (left > 32) m |= uint64_t(w[1]) << 32;
-    if (left < 64) m |= ~0ull << left;
-    return m;
 }
 
 // What one block of rows works on.
@@ -222,13 +205,13 @@ __global__ void __launch_bounds__(PR_THREADS) paged_rows_kernel(const PagedAtten
             for (int n = 0; n < NT; ++n) m = fmaxf(m, fmaxf(sc[n][2 * j], sc[n][2 * j + 1]));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-            const float ref = m == -INFINITY ? 0.f : m, f = exp2_fast(mx[j] - ref);
+            const float ref = m == -INFINITY ? 0.f : m, f = exp2_ftz(mx[j] - ref);
             mx[j] = m;
             float ps = 0.f;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                sc[n][2 * j] = exp2_fast(sc[n][2 * j] - ref);
-                sc[n][2 * j + 1] = exp2_fast(sc[n][2 * j + 1] - ref);
+                sc[n][2 * j] = exp2_ftz(sc[n][2 * j] - ref);
+                sc[n][2 * j + 1] = exp2_ftz(sc[n][2 * j + 1] - ref);
                 ps += sc[n][2 * j] + sc[n][2 * j + 1];
             }
             sum[j] = fmaf(sum[j], f, ps);
@@ -282,7 +265,7 @@ __global__ void __launch_bounds__(PR_THREADS) paged_rows_kernel(const PagedAtten
         for (int k = 0; k < KG; ++k) {
             const int w = k * RG + g;
             const float2 ml = sml[w * 16 + rr];
-            const float f = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - m);
+            const float f = ml.x == -INFINITY ? 0.f : exp2_ftz(ml.x - m);
             l = fmaf(ml.y, f, l);
             const float* src = reinterpret_cast<const float*>(smem) + w * 16 * HD + rr * HD + ((c ^ (rr & 7)) << 3);
 #pragma unroll
@@ -331,7 +314,7 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttention
     for (int s = 0; s < a.splits; ++s) {
         const float2 ml = a.part_ml[s * step + at];
         if (ml.x == -INFINITY) continue;              // saw nothing: no partial row was written
-        const float f = exp2_fast(ml.x - m);
+        const float f = exp2_ftz(ml.x - m);
         l = fmaf(ml.y, f, l);
         const float4* src = reinterpret_cast<const float4*>(a.part_o + (s * step + at) * HD + c * 8);
         const float4 u = src[0], w = src[1];
@@ -393,9 +376,13 @@ cudaError_t launch_combine(const PagedAttention& a, cudaStream_t stream) {
 
 template <class T, int HD>
 cudaError_t dispatch(const PagedAttention& a, cudaStream_t stream) {
-    const int rg = rows_group(a);
-    const cudaError_t e = rg == 1 ? launch_rows<T, HD, 1>(a, stream) : rg == 2 ? launch_rows<T, HD, 2>(a, stream)
-                                                                              : launch_rows<T, HD, 4>(a, stream);
+    bool taken = false;
+    cudaError_t e = cudaSuccess;
+    if (paged_plan(a).tiles) e = paged_attention_tiles(a, std::is_same<T, __nv_bfloat16>::value, stream, &taken);
+    if (!taken) {
+        const int rg = rows_group(a);
+        e = rg == 1 ? launch_rows<T, HD, 1>(a, stream) : rg == 2 ? launch_rows<T, HD, 2>(a, stream) : launch_rows<T, HD, 4>(a, stream);
+    }
     if (e != cudaSuccess || a.splits == 1) return e;
     return launch_combine<T, HD>(a, stream);
 }
@@ -404,11 +391,12 @@ cudaError_t dispatch(const PagedAttention& a, cudaStream_t stream) {
 
 PagedPlan paged_plan(const PagedAttention& a) {
     PagedPlan p;
-    const int mt = 16 * rows_group(a);
+    p.tiles = int64_t(a.batch.max_chunk) * a.group > 64;
+    const int mt = p.tiles ? kPagedTileRows : 16 * rows_group(a), tile = p.tiles ? 128 : 64;
     const int64_t blocks = (int64_t(a.batch.max_chunk) * a.group + mt - 1) / mt * a.cache.kv_heads * a.batch.seqs;
     const int keys = a.window ? int(std::min<int64_t>(a.batch.max_length, int64_t(a.window) + a.batch.max_chunk)) : a.batch.max_length;
-    const int64_t want = int64_t(device_sm_count()) * 2;
-    p.splits = int(std::max<int64_t>(1, std::min<int64_t>({(want + blocks - 1) / blocks, (keys + 255) / 256, 256})));
+    const int64_t want = int64_t(device_sm_count()) * (p.tiles ? 1 : 2);
+    p.splits = int(std::max<int64_t>(1, std::min<int64_t>({(want + blocks - 1) / blocks, (keys + 4 * tile - 1) / (4 * tile), 256})));
     p.split_bytes = size_t(a.batch.tokens) * a.q_heads * (size_t(a.cache.head_dim) * 4 + 8);
     return p;
 }

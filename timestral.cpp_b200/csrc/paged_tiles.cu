@@ -1,0 +1,427 @@
+// Attention of new tokens over a paged cache, many rows: prompts and long chunks on tcgen05.
+//
+// A block owns 256 rows (token, query head of the group) of one (sequence, cached head) as two
+// tiles of 128 and streams the keys and values that they see in tiles of 128, so that a tile in
+// shared memory serves both row tiles. Warps 0-3 and 4-7 hold the two row tiles, a thread a row
+// (TMEM lane); warp 8 issues the MMAs, warp 9 the TMA loads, one per page that the tile touches.
+// TMEM (512 columns): the scores S of each row tile (128 columns), which its f16 probabilities
+// overwrite (two keys a column), and its weighted values O. The MMAs of one row tile run while
+// the other's softmax does: per key tile, in the order of issue and so of execution,
+//   O0 += P0 V_j, S0 = Q0 K_{j+1}, O1 += P1 V_j, S1 = Q1 K_{j+1}.
+// A commit covers every earlier MMA, so a full S_{j+1} also says that O holds tile j: the softmax
+// may rescale it. It does so only when a row's maximum passes its reference by more than 2^8
+// (probabilities then lie in (0, 256]).
+#include "paged.cuh"
+
+#include <algorithm>
+#include <climits>
+
+namespace tsb {
+
+bool make_map_4d_16bit(CUtensorMap* map, const void* base, bool bf16, int width, const int64_t (&size)[3],
+                       const int64_t (&stride)[3], const int (&box_rows)[3]);
+int device_sm_count();
+
+namespace {
+
+constexpr int PT_THREADS = 320;
+constexpr int PT_KT = 128;
+constexpr uint32_t PT_TMEM = 512, PT_O_COL = 256;
+constexpr float PT_RESCALE = 8.f;       // log2 of the largest probability kept unscaled
+
+template <int HD>
+struct TilesLayout {
+    static constexpr int HALF = 128 * 128;                       // 128 rows of 64 values
+    static constexpr int SLOT = HD / 64 * HALF;                  // a key tile, a value tile or a row tile
+    static constexpr int STAGES = HD == 64 ? 8 : 5;
+    static constexpr int SMEM = 1024 + (2 + STAGES) * SLOT + 256;
+};
+
+struct TilesBars {
+    uint64_t full[8], empty[8], q_ready[2], s_full[2], p_ready[2], o_full[2];
+    uint32_t tmem;
+    int abort;
+};
+static_assert(sizeof(TilesBars) <= 256);
+
+// Which coordinate of a cache's tensor map stands for what (its axes are in order of stride).
+struct PageMap {
+    int slot, head, page;               // 1, 2 or 3
+};
+__device__ __forceinline__ void load_page(void* dst, const CUtensorMap* map, uint64_t* bar, const PageMap& m, int x, int slot,
+                                          int head, int page) {
+    const int c1 = m.slot == 1 ? slot : m.head == 1 ? head : page;
+    const int c2 = m.slot == 2 ? slot : m.head == 2 ? head : page;
+    const int c3 = m.slot == 3 ? slot : m.head == 3 ? head : page;
+    tma_load_4d(dst, map, bar, x, c1, c2, c3);
+}
+
+// Bits [lo, hi] (inclusive, any ints) of the 32-bit word that starts at bit w0.
+__device__ __forceinline__ uint32_t range32(int lo, int hi, int w0) {
+    lo = max(lo - w0, 0);
+    hi = min(hi - w0, 31);
+    if (lo > hi) return 0u;
+    return (0xffffffffu >> (31 - hi)) & (0xffffffffu << lo);
+}
+
+template <class T, int HD>
+__global__ void __launch_bounds__(PT_THREADS, 1)
+    paged_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PageMap mk,
+                       const PageMap mv, const PagedAttention a, int row_tiles) {
+    using L = TilesLayout<HD>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* qbuf = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* ring = qbuf + 2 * L::SLOT;
+    TilesBars* bars = reinterpret_cast<TilesBars*>(ring + L::STAGES * L::SLOT);
+    volatile int* abort = &bars->abort;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+    // the block's rows; the row tiles that see most keys come first
+    const int split = int(blockIdx.x % a.splits);
+    int b = int(blockIdx.x / a.splits);
+    const int per = a.cache.kv_heads * a.batch.seqs;
+    const int m0 = (row_tiles - 1 - b / per) * kPagedTileRows;
+    b %= per;
+    const int kvh = b % a.cache.kv_heads, seq = b / a.cache.kv_heads;
+    const SeqInfo q = load_seq(a.batch, seq, a.err);
+    const int rows = min(kPagedTileRows, q.n * a.group - m0);
+    if (rows <= 0) return;
+    const int base = q.len - q.n;
+    auto position = [&](int r) { return base + (m0 + r) / a.group; };
+    const int hi = position(rows - 1) + 1;
+    const int lo = a.window ? max(0, position(0) - a.window + 1) : 0;
+    const int tile0 = lo / PT_KT, tiles = (hi + PT_KT - 1) / PT_KT - tile0;
+    const int share = (tiles + a.splits - 1) / a.splits;
+    const int first = tile0 + split * share, n = min(share, tile0 + tiles - first);
+    // key tiles of each row tile in this block's share
+    int ng[2];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+        const int last_row = min(rows, (g + 1) * 128) - 1;
+        ng[g] = last_row < g * 128 || n <= 0 ? 0 : min(n, max(0, (position(last_row) + PT_KT) / PT_KT - first));
+    }
+    const int nt = max(ng[0], ng[1]);
+
+    const int t = threadIdx.x & 127, g = threadIdx.x >> 7;         // (warps 0-7)
+    const int row = g * 128 + t;
+    const bool live = warp < 8 && row < rows;
+    const int64_t token = q.start + (m0 + row) / a.group;
+    const int head = kvh * a.group + (m0 + row) % a.group;
+    const int64_t part = (int64_t(split) * a.batch.tokens + token) * a.q_heads + head;
+    if (nt == 0) {                                                  // (only with splits)
+        if (live) a.part_ml[part] = make_float2(-INFINITY, 0.f);
+        return;
+    }
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < L::STAGES; ++s) { mbar_init(&bars->full[s], 1); mbar_init(&bars->empty[s], 1); }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bars->q_ready[i], 4); mbar_init(&bars->s_full[i], 1);
+            mbar_init(&bars->p_ready[i], 4); mbar_init(&bars->o_full[i], 1);
+        }
+        bars->abort = 0;
+        mbar_fence_init();
+        fence_proxy_async();
+    }
+    if (warp == 8) { tmem_alloc(&bars->tmem, PT_TMEM); tmem_relinquish(); }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tbase = bars->tmem;
+
+    if (warp == 9) {
+        // TMA producer: K_0, V_0, K_1, V_1, ... through one ring; lane p loads page piece p of a tile.
+        const int slots = 1 << a.cache.page_shift, box = min(slots, PT_KT);
+        const int* table = a.cache.table + int64_t(seq) * a.cache.table_stride;
+        const int key0 = first * PT_KT + lane * box;
+        auto page_of = [&](int j) {
+            const int key = key0 + j * PT_KT;
+            if (lane * box >= PT_KT || j >= nt || key + box <= lo || key >= hi) return -1;
+            const int page = table[key >> a.cache.page_shift];
+            if (page >= 0 && page < a.cache.num_pages) return page;
+            record_error(a.err, kDevBadPage);
+            return a.cache.num_pages;                              // outside the map: zeros
+        };
+        int next = page_of(0), page = -1;
+        for (int i = 0; i < 2 * nt; ++i) {
+            const int j = i >> 1, s = i % L::STAGES;
+            if ((i & 1) == 0) { page = next; next = page_of(j + 1); }
+            if (i >= L::STAGES && !warp_wait(&bars->empty[s], ((i / L::STAGES) - 1) & 1, abort, a.err)) break;
+            const int pieces = __popc(__ballot_sync(0xffffffffu, page >= 0));
+            if (lane == 0) mbar_arrive_expect_tx(&bars->full[s], pieces * box * HD * 2);
+            __syncwarp();
+            if (page >= 0) {
+                const int slot = (key0 + j * PT_KT) & (slots - 1);
+                uint8_t* dst = ring + s * L::SLOT + lane * box * 128;
+#pragma unroll
+                for (int h = 0; h < HD / 64; ++h)
+                    load_page(dst + h * L::HALF, (i & 1) ? &map_v : &map_k, &bars->full[s], (i & 1) ? mv : mk, h * 64, slot, kvh, page);
+            }
+            __syncwarp();
+        }
+    } else if (warp == 8) {
+        if (lane == 0) {
+            constexpr uint32_t bf = std::is_same<T, __nv_bfloat16>::value ? kIdescBf16 : 0u;
+            const uint32_t id_qk = idesc_f16(128, PT_KT) | bf, id_pv = idesc_f16_bmn(128, HD) | bf;
+            auto scores = [&](int gg, int j) {                      // S_gg = Q_gg K_j
+                const uint64_t dq = smem_desc_sw128(smem_u32(qbuf + gg * L::SLOT));
+                const uint64_t dk = smem_desc_sw128(smem_u32(ring + (2 * j) % L::STAGES * L::SLOT));
+#pragma unroll
+                for (int k = 0; k < HD / 16; ++k) {
+                    const uint64_t off = uint64_t((k / 4) * (L::HALF >> 4) + (k % 4) * 2);
+                    mma_f16(tbase + gg * 128, dq + off, dk + off, id_qk, k > 0);
+                }
+                mma_commit(&bars->s_full[gg]);
+            };
+            auto full = [&](int i) { return at_wait(&bars->full[i % L::STAGES], (i / L::STAGES) & 1, abort, a.err); };
+            auto release = [&](int i) { mma_commit(&bars->empty[i % L::STAGES]); };
+            bool ok = full(0);
+#pragma unroll
+            for (int gg = 0; gg < 2; ++gg)
+                if (ok && ng[gg] > 0) {
+                    ok = at_wait(&bars->q_ready[gg], 0, abort, a.err);
+                    tc_fence_after();
+                    if (ok) scores(gg, 0);
+                }
+            if (ok) release(0);
+            for (int j = 0; j < nt && ok; ++j) {
+                ok = full(2 * j + 1);
+                const uint32_t sv = smem_u32(ring + (2 * j + 1) % L::STAGES * L::SLOT);
+                bool have_k = false;
+#pragma unroll
+                for (int gg = 0; gg < 2; ++gg) {
+                    if (ok && j < ng[gg]) {
+                        ok = at_wait(&bars->p_ready[gg], j & 1, abort, a.err);
+                        tc_fence_after();
+                        if (ok) {
+#pragma unroll
+                            for (int kk = 0; kk < PT_KT / 16; ++kk)
+                                mma_f16_ts(tbase + PT_O_COL + gg * 128, tbase + gg * 128 + kk * 8,
+                                           smem_desc_sw128_mn(sv + kk * 16 * 128, L::HALF), id_pv, j > 0 || kk > 0);
+                            if (j + 1 == ng[gg]) mma_commit(&bars->o_full[gg]);
+                        }
+                    }
+                    if (ok && gg == 1) release(2 * j + 1);
+                    if (ok && j + 1 < ng[gg]) {
+                        if (!have_k) ok = full(2 * j + 2);
+                        have_k = true;
+                        tc_fence_after();
+                        if (ok) scores(gg, j + 1);
+                    }
+                }
+                if (ok && j + 1 < nt) release(2 * j + 2);
+            }
+        }
+        __syncwarp();
+    } else {
+        // Softmax of row `row`, a thread of TMEM lane t.
+        const int ngg = g ? ng[1] : ng[0];
+        const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
+        const uint32_t ts = tbase + lanes + g * 128, to = tbase + lanes + PT_O_COL + g * 128;
+        const int pos = live ? position(row) : -1;
+        const int rows_g = min(rows - g * 128, 128);
+        const int pos_first = position(g * 128), pos_last = rows_g > 0 ? position(g * 128 + rows_g - 1) : -1;
+        const int from = a.window ? pos - a.window + 1 : 0;         // the row sees positions from .. pos
+        const float scale = fabsf(a.scale_log2);
+        if (ngg > 0) {
+            // the row tile goes to shared memory by its threads (any strides); with a negative scale its
+            // signs turn, so that the largest product has the largest score
+            const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+            const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q.data) + token * a.q.token + head * a.q.head);
+#pragma unroll
+            for (int c = 0; c < HD / 8; ++c) {
+                uint4 u = live ? src[c] : make_uint4(0, 0, 0, 0);
+                u.x ^= flip; u.y ^= flip; u.z ^= flip; u.w ^= flip;
+                *reinterpret_cast<uint4*>(qbuf + g * L::SLOT + (c / 8) * L::HALF + t * 128 + (((c & 7) ^ (t & 7)) << 4)) = u;
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->q_ready[g]);
+        }
+        float mref = -INFINITY, sum = 0.f;
+        bool ok = true;
+        for (int j = 0; j < ngg; ++j) {
+            const int k0 = (first + j) * PT_KT;
+            uint64_t v01 = ~0ull, v23 = ~0ull;
+            if (a.key_valid) { v01 = valid_bits(a, seq, k0); v23 = valid_bits(a, seq, k0 + 64); }
+            const bool dead_keys = k0 < lo || k0 + PT_KT > hi || (v01 & v23) != ~0ull;
+            const bool plain = k0 + PT_KT - 1 <= pos_first && (!a.window || k0 > pos_last - a.window) && (v01 & v23) == ~0ull;
+            if (dead_keys && g == (j < ng[0] ? 0 : 1)) {
+                // values of keys that no row of the block sees: zeros instead of what stands there
+                const int i = 2 * j + 1;
+                if (!(ok = warp_wait(&bars->full[i % L::STAGES], (i / L::STAGES) & 1, abort, a.err))) break;
+                const int key = k0 + t;
+                const bool valid = ((t < 64 ? v01 >> t : v23 >> (t - 64)) & 1) || (a.self_visible && key >= base);
+                if (key < lo || key >= hi || !valid) {
+                    uint8_t* v = ring + i % L::STAGES * L::SLOT + t * 128;
+#pragma unroll
+                    for (int h = 0; h < HD / 64; ++h)
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(v + h * L::HALF + (((c + t) & 7) << 4)) = make_uint4(0, 0, 0, 0);
+                }
+                fence_proxy_async();
+            }
+            if (!(ok = warp_wait(&bars->s_full[g], j & 1, abort, a.err))) break;
+            tc_fence_after();
+            uint32_t s[4][32];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, s[c]);
+            tmem_ld_wait();
+            if (!plain) {
+                const uint32_t vw[4] = {uint32_t(v01), uint32_t(v01 >> 32), uint32_t(v23), uint32_t(v23 >> 32)};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const int w0 = k0 + c * 32;
+                    const uint32_t see = (vw[c] & range32(from, pos, w0)) | (a.self_visible ? range32(pos, pos, w0) : 0u);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        if (!((see >> e) & 1u)) s[c][e] = __float_as_uint(-INFINITY);
+                }
+            }
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int e = 0; e < 32; e += 2)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) mx[c] = fmaxf(fmaxf(mx[c], __uint_as_float(s[c][e])), __uint_as_float(s[c][e + 1]));
+            const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+            const bool need = mref != -INFINITY && mt > mref + PT_RESCALE;
+            float factor = 1.f;
+            if (need) { factor = exp2_ftz(mref - mt); sum *= factor; }
+            if (need || mref == -INFINITY) mref = mt;
+            if (__any_sync(0xffffffffu, need)) {
+#pragma unroll 1
+                for (int c0 = 0; c0 < HD; c0 += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(to + c0, o);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * factor);
+                    tmem_st32(to + c0, o);
+                }
+            }
+            const float off = mref == -INFINITY ? 0.f : mref;
+            float ps[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                uint32_t pk[32];
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                    const int c = half * 2 + e / 16, k = (e % 16) * 2;
+                    const float e0 = exp2_ftz(__fmaf_rn(__uint_as_float(s[c][k]), scale, -off));
+                    const float e1 = exp2_ftz(__fmaf_rn(__uint_as_float(s[c][k + 1]), scale, -off));
+                    ps[e & 3] += e0 + e1;
+                    pk[e] = Pair<T>::down(e0, e1);
+                }
+                tmem_st32(ts + half * 32, pk);
+            }
+            sum += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->p_ready[g]);
+        }
+        if (ok && ngg > 0) ok = warp_wait(&bars->o_full[g], 0, abort, a.err);
+        if (ok) {
+            tc_fence_after();
+            const bool none = ngg == 0;
+            if (a.splits > 1 && live) a.part_ml[part] = none ? make_float2(-INFINITY, 0.f) : make_float2(mref, sum);
+            const float inv = none || mref == -INFINITY ? 0.f : a.splits > 1 ? 1.f : 1.0f / sum;
+            const T* gate = a.gate.data ? static_cast<const T*>(a.gate.data) + token * a.gate.token + head * a.gate.head : nullptr;
+            T* out = static_cast<T*>(a.out.data) + token * a.out.token + head * a.out.head;
+#pragma unroll 1
+            for (int c0 = 0; c0 < HD; c0 += 32) {
+                uint32_t o[32];
+                if (none) {
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) o[c] = 0u;
+                } else {
+                    tmem_ld32(to + c0, o);
+                    tmem_ld_wait();
+                }
+                if (!live) continue;
+                if (a.splits > 1) {
+                    if (none) continue;
+                    float4* dst = reinterpret_cast<float4*>(a.part_o + part * HD + c0);
+#pragma unroll
+                    for (int c = 0; c < 8; ++c)
+                        dst[c] = make_float4(__uint_as_float(o[4 * c]), __uint_as_float(o[4 * c + 1]), __uint_as_float(o[4 * c + 2]),
+                                             __uint_as_float(o[4 * c + 3]));
+                    continue;
+                }
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float y[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[e] = __uint_as_float(o[8 * c + e]) * inv;
+                    if (gate) {
+                        float gt[8];
+                        unpack8<T>(*reinterpret_cast<const uint4*>(gate + c0 + 8 * c), gt);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) y[e] *= gt[e];
+                    }
+                    *reinterpret_cast<uint4*>(out + c0 + 8 * c) = pack8<T>(y);
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 8) tmem_dealloc(tbase, PT_TMEM);
+}
+
+// A tensor map over one of the pools, its axes in order of stride (an axis of one entry has none of
+// its own), in boxes of `box` slots.
+bool page_map(CUtensorMap* map, PageMap* at, const void* base, bool bf16, const PagedCache& c, int64_t page, int64_t head,
+              int64_t slot) {
+    const int slots = 1 << c.page_shift;
+    struct Axis { int64_t stride, size; int box; int* where; } ax[3] = {{slot, slots, std::min(slots, PT_KT), &at->slot},
+                                                                        {head, c.kv_heads, 1, &at->head},
+                                                                        {page, c.num_pages, 1, &at->page}};
+    int64_t top = 0;
+    for (const Axis& x : ax) top = std::max(top, x.size > 1 ? x.stride * x.size : x.stride);
+    for (Axis& x : ax)
+        if (x.size == 1) x.stride = top;
+    std::stable_sort(ax, ax + 3, [](const Axis& x, const Axis& y) { return x.stride < y.stride; });
+    for (int i = 0; i < 3; ++i) *ax[i].where = i + 1;
+    return make_map_4d_16bit(map, base, bf16, c.head_dim, {ax[0].size, ax[1].size, ax[2].size},
+                             {ax[0].stride, ax[1].stride, ax[2].stride}, {ax[0].box, ax[1].box, ax[2].box});
+}
+
+template <class T, int HD>
+cudaError_t launch_tiles(const PagedAttention& a, cudaStream_t stream, bool* taken) {
+    using L = TilesLayout<HD>;
+    constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+    *taken = false;
+    const PagedCache& c = a.cache;
+    CUtensorMap map_k, map_v;
+    PageMap mk, mv;
+    if (!page_map(&map_k, &mk, c.k, bf16, c, c.k_page, c.k_head, c.k_slot) ||
+        !page_map(&map_v, &mv, c.v, bf16, c, c.v_page, c.v_head, c.v_slot))
+        return cudaSuccess;
+    *taken = true;
+    static KernelSetup configured;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    unsigned long long key = 0;
+    if (configured.needed(dev, &key)) {
+        const cudaError_t e = cudaFuncSetAttribute(paged_tiles_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
+        if (e != cudaSuccess) return e;
+        configured.done(dev, key);
+    }
+    const int64_t row_tiles = (int64_t(a.batch.max_chunk) * a.group + kPagedTileRows - 1) / kPagedTileRows;
+    const int64_t blocks = row_tiles * c.kv_heads * a.batch.seqs * a.splits;
+    if (blocks > INT32_MAX) return cudaErrorInvalidValue;
+    paged_tiles_kernel<T, HD><<<unsigned(blocks), PT_THREADS, L::SMEM, stream>>>(map_k, map_v, mk, mv, a, int(row_tiles));
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t paged_attention_tiles(const PagedAttention& a, bool bf16, cudaStream_t stream, bool* taken) {
+    if (a.cache.head_dim == 64)
+        return bf16 ? launch_tiles<__nv_bfloat16, 64>(a, stream, taken) : launch_tiles<__half, 64>(a, stream, taken);
+    return bf16 ? launch_tiles<__nv_bfloat16, 128>(a, stream, taken) : launch_tiles<__half, 128>(a, stream, taken);
+}
+
+}  // namespace tsb

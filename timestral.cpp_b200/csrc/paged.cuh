@@ -81,6 +81,7 @@ struct PagedAttention {
 // the call agree. splits is what it would like without a bound on the workspace.
 struct PagedPlan {
     bool tiles = false;                 // paged_attention_tiles, else paged_attention_rows
+    bool join = false;                  // rows: a block's teams share one problem
     int splits = 1;
     size_t split_bytes = 0;             // workspace bytes of one split
 };
@@ -90,13 +91,33 @@ PagedPlan paged_plan(const PagedAttention& a);
 cudaError_t norm_rope(const NormRope& a, bool bf16, cudaStream_t stream);
 cudaError_t paged_append(const PagedAppend& a, bool bf16, cudaStream_t stream);
 cudaError_t paged_attention(const PagedAttention& a, bool bf16, cudaStream_t stream);
-// The kernel for many rows (paged_tiles.cu): *taken is false, and nothing was launched, when the
-// cache's strides do not fit a tensor map.
-cudaError_t paged_attention_tiles(const PagedAttention& a, bool bf16, cudaStream_t stream, bool* taken);
+// The kernel for many rows (paged_tiles.cu).
+cudaError_t paged_attention_tiles(const PagedAttention& a, bool bf16, cudaStream_t stream);
 constexpr int kPagedTileRows = 256;     // its rows per block
+
+// A tensor map over one of the cache's pools: 64 values by up to box_slots slots of one head and
+// page, and which coordinate (1, 2 or 3) stands for what, its axes being in order of stride.
+struct PageMap {
+    CUtensorMap map;
+    int slot, head, page;
+};
+struct PageMaps {
+    PageMap k, v;
+};
+// false when the cache's strides do not fit a tensor map.
+bool page_maps(PageMaps* m, const PagedCache& c, bool bf16, int box_slots);
 
 // ---------------------------------------------------------------------------------------
 // Device helpers
+
+// 64 values (from x, a multiple of 64) of a box of slots: rows of 128 bytes at dst, 128-byte
+// swizzle. A page number outside the pool gives zeros.
+__device__ __forceinline__ void load_page(void* dst, const PageMap& m, uint64_t* bar, int x, int slot, int head, int page) {
+    const int c1 = m.slot == 1 ? slot : m.head == 1 ? head : page;
+    const int c2 = m.slot == 2 ? slot : m.head == 2 ? head : page;
+    const int c3 = m.slot == 3 ? slot : m.head == 3 ? head : page;
+    tma_load_4d(dst, &m.map, bar, x, c1, c2, c3);
+}
 
 // The new tokens of sequence s, checked against the bounds the host gave; a contradiction is
 // recorded and gives ok = false.

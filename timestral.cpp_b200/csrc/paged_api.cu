@@ -103,6 +103,7 @@ bool batch_shape(Refusal& r, const tsb_paged_batch* b, const tsb_paged_cache* c,
     return r.need(b != nullptr, "batch is NULL") &&
            r.need(b->seqs >= 0 && b->max_chunk >= 0 && b->max_length >= 0 && tokens >= 0, "a size is negative") &&
            aligned(r, b->q_start, "q_start", 4) && aligned(r, b->lengths, "lengths", 4) &&
+           r.need(b->max_length <= INT_MAX - 1024, "max_length %d is above 2^31 - 1025", b->max_length) &&
            r.need(int64_t(b->max_length) <= int64_t(c->table_width) * c->page_size,
                   "max_length %d is more than the page table holds (%d pages of %d)", b->max_length, c->table_width, c->page_size);
 }
@@ -130,7 +131,8 @@ tsb::PagedCache view(const tsb_paged_cache& c) {
 }
 tsb::PagedBatch view(const tsb_paged_batch& b, int tokens) {
     tsb::PagedBatch v;
-    v.q_start = b.q_start; v.lengths = b.lengths; v.seqs = b.seqs; v.max_chunk = b.max_chunk; v.max_length = b.max_length;
+    v.q_start = b.q_start; v.lengths = b.lengths; v.seqs = b.seqs; v.max_length = b.max_length;
+    v.max_chunk = b.max_chunk < tokens ? b.max_chunk : tokens;      // more than there are cannot be
     v.tokens = tokens;
     return v;
 }
@@ -149,7 +151,7 @@ bool error_word(Refusal& r, int32_t* error, int dev) {
 
 int launched(Refusal& r, cudaError_t e) {
     if (e == cudaSuccess) return TSB_OK;
-    std::snprintf(r.text, sizeof(r.text), "%s: %s", r.call, e == cudaErrorInvalidValue ? "too many blocks for one launch" : cudaGetErrorString(e));
+    std::snprintf(r.text, sizeof(r.text), "%s: %s", r.call, e == cudaErrorInvalidValue ? "a size or stride that does not fit a launch or a tensor map" : cudaGetErrorString(e));
     cudaGetLastError();
     r.code = e == cudaErrorInvalidValue ? TSB_ERR_ARG : TSB_ERR_CUDA;
     return r.report();
@@ -168,6 +170,7 @@ bool attention_shape(Refusal& r, const tsb_paged_attention_args* a, bool pointer
     if (!r.need(a != nullptr, "args is NULL") || !cache_shape(r, a->cache) || !batch_shape(r, a->batch, a->cache, a->tokens)) return false;
     const tsb_paged_cache& c = *a->cache;
     if (!r.need(a->q_heads > 0 && a->q_heads % c.kv_heads == 0, "q_heads %d is not a multiple of kv_heads %d", a->q_heads, c.kv_heads) ||
+        !r.need(int64_t(a->tokens) * a->q_heads <= INT_MAX, "%d tokens of %d heads are more than 2^31 - 1 rows", a->tokens, a->q_heads) ||
         !r.need(a->window >= 0, "window %d is negative", a->window))
         return false;
     return !pointers ||

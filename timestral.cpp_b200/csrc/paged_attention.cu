@@ -12,24 +12,38 @@
 
 namespace tsb {
 
+bool make_map_4d_16bit(CUtensorMap* map, const void* base, bool bf16, int width, const int64_t (&size)[3],
+                       const int64_t (&stride)[3], const int (&box_rows)[3]);
 int device_sm_count();
 
 namespace {
 
 // ---------------------------------------------------------------------------------------
-// Few rows (single tokens, short chunks): 16 * RG rows a block on mma.sync, bound by the bytes of
-// the cache. Four warps: RG row groups of 16 rows, 4 / RG key groups that share each 64-key tile
-// out; tiles come in a ring by 16-byte cp.async, in which a key that no row sees (behind the
-// length, outside the window, its bit clear) is filled with zeros and not read, so that neither
-// its bytes nor what stands there matter. tcgen05 would pad 16 rows to 128 and has nothing to win.
+// Few rows (single tokens, short chunks) on mma.sync, bound by the bytes of the cache. The products
+// are taken transposed, S^T = K Q^T and O^T = V^T P^T: keys and values fill the 16 rows of the MMA
+// and the rows of the problem its 8 columns, so that the one to eight rows of a decoded token pad
+// to 8, not to 16 (half the MMAs and exponentials) or to the 128 of tcgen05.
+// A warp owns 8 * NR rows. RG warps form a team of 8 * NR * RG rows that streams tiles of keys and
+// values through a ring of its own; a block's teams work on different problems (short rows:
+// nothing to join), or with JOIN on the tiles of one problem in turn, joined through shared
+// memory at the end.
+// Tiles come by TMA, a load for each page that they touch (a 16-byte cp.async path cost 350
+// instructions a tile and ran at 0.57 of the copy rate, a bulk copy for each row, 40 cycles each,
+// at 0.27). What stands at keys that no row sees (behind the length, outside the window, the bit
+// clear) is masked in the scores, and the values there are overwritten with zeros.
 constexpr int PR_THREADS = 128;
-constexpr int PR_KT = 64;
+constexpr float PR_RESCALE = 8.f;        // log2 of the largest probability kept unscaled
 
-template <int HD>
+template <int HD, int RG>
 struct RowsLayout {
-    static constexpr int STAGES = HD == 64 ? 4 : 3;
-    static constexpr int TILE = PR_KT * HD * 2;             // bytes of one tile of keys (or values)
-    static constexpr int SMEM = STAGES * 2 * TILE;
+    static constexpr int TEAMS = 4 / RG;
+    static constexpr int KT = RG == 4 ? 64 : 32;            // keys of a tile: one or two copies a lane
+    static constexpr int STAGES = 3;
+    static constexpr int HALF = KT * 128;                   // 64 values of the tile's keys
+    static constexpr int TILE = HD / 64 * HALF;             // bytes of a tile of keys (or values)
+    static constexpr int RING = STAGES * 2 * TILE;
+    static constexpr int SMEM = 1024 + TEAMS * RING + TEAMS * STAGES * 8;
+    static_assert(SMEM >= 4 * 16 * HD * 4 + 4 * 16 * 8, "the joined rows reuse the rings");
 };
 
 template <class T>
@@ -50,231 +64,418 @@ __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
+// An 8 x 8 block of 16-bit values, held by a warp as a fragment, turned over.
+__device__ __forceinline__ uint32_t turn8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
 __device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-// 16 bytes, or zeros without reading `src`.
-__device__ __forceinline__ void cp_async16_if(uint32_t dst, const void* src, bool read) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(read ? 16 : 0) : "memory");
+// All warps of a team (a warp alone: the warp).
+template <int RG>
+__device__ __forceinline__ void team_sync(int team) {
+    if constexpr (RG == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(32 * RG) : "memory");
 }
 
-// What one block of rows works on.
+// Division by a number known at launch: n / d for n < 2^31 as the high word of a product.
+struct FastDiv {
+    uint32_t d = 1, mul = 0, shift = 0;
+    FastDiv() = default;
+    explicit FastDiv(uint32_t divisor) : d(divisor) {
+        if (d == 1) return;
+        while ((1ull << shift) < d) ++shift;                       // mul = ceil(2^(31 + shift) / d) < 2^32
+        mul = uint32_t(((1ull << (31 + shift)) + d - 1) / d);
+        --shift;
+    }
+    __device__ __forceinline__ uint32_t div(uint32_t n) const { return d == 1 ? n : __umulhi(n, mul) >> shift; }
+    __device__ __forceinline__ uint32_t divmod(uint32_t n, uint32_t* rest) const {
+        const uint32_t x = div(n);
+        *rest = n - x * d;
+        return x;
+    }
+};
+struct RowsGrid {
+    FastDiv splits, heads, row_tiles, group;
+    uint32_t items = 0;
+};
+
+// What a team works on.
 struct RowTile {
     int seq, kvh, m0, rows;      // first row and live rows of the tile
     int base;                    // position of the sequence's first new token
     int lo, hi;                  // keys that any row of the tile may see
-    int len;                     // length of the sequence
     int start;                   // first token row
 };
 
-template <class T, int HD>
-__device__ __forceinline__ void load_tile(const PagedAttention& a, const RowTile& t, int k0, uint32_t sk, uint32_t sv) {
-    constexpr int CH = HD / 8, STEP = PR_THREADS / CH;
-    const PagedCache& c = a.cache;
-    const int chunk = threadIdx.x % CH;
-    const uint64_t valid = valid_bits(a, t.seq, k0);
-    const int slots = 1 << c.page_shift;
-    const int* table = c.table + int64_t(t.seq) * c.table_stride;
+// Eight finished values (columns 8 c ..) of a row: normalised, gated, rounded, stored.
+template <class T>
+__device__ __forceinline__ void store_row(const PagedAttention& a, int64_t token, int head, int c, float (&y)[8], float inv) {
 #pragma unroll
-    for (int i = 0; i < PR_KT / STEP; ++i) {
-        const int r = threadIdx.x / CH + i * STEP, key = k0 + r;
-        bool read = key >= t.lo && key < t.hi && (((valid >> r) & 1) || (a.self_visible && key >= t.base));
-        int page = 0;
-        if (read) {
-            page = table[key >> c.page_shift];
-            if (page < 0 || page >= c.num_pages) { record_error(a.err, kDevBadPage); read = false; page = 0; }
-        }
-        const int slot = key & (slots - 1);
-        const T* k = static_cast<const T*>(c.k) + page * c.k_page + t.kvh * c.k_head + slot * c.k_slot + chunk * 8;
-        const T* v = static_cast<const T*>(c.v) + page * c.v_page + t.kvh * c.v_head + slot * c.v_slot + chunk * 8;
-        const uint32_t at = uint32_t(r * HD * 2 + ((chunk ^ (r & 7)) << 4));
-        cp_async16_if(sk + at, k, read);
-        cp_async16_if(sv + at, v, read);
+    for (int e = 0; e < 8; ++e) y[e] *= inv;
+    if (a.gate.data) {
+        float g[8];
+        unpack8<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(a.gate.data) + token * a.gate.token + head * a.gate.head + c * 8), g);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] *= g[e];
     }
+    *reinterpret_cast<uint4*>(static_cast<T*>(a.out.data) + token * a.out.token + head * a.out.head + c * 8) = pack8<T>(y);
 }
 
-// Whether the token at position pos sees key.
-__device__ __forceinline__ bool sees(const PagedAttention& a, int key, int pos, bool valid) {
-    return key <= pos && (a.window == 0 || key > pos - a.window) && (valid || (a.self_visible && key == pos));
+// Four 32-bit values a lane, one for each of four 8-value columns of a row that the quad shares:
+// afterwards lane i of the quad holds all of column i.
+__device__ __forceinline__ void quad_transpose(uint32_t (&v)[4]) {
+    const int i = threadIdx.x & 3;
+    const bool odd = i & 1, high = i & 2;
+    // lane i exchanges with i ^ 1, then with i ^ 2
+    uint32_t a = __shfl_xor_sync(0xffffffffu, odd ? v[0] : v[1], 1), b = __shfl_xor_sync(0xffffffffu, odd ? v[2] : v[3], 1);
+    if (odd) { v[0] = a; v[2] = b; } else { v[1] = a; v[3] = b; }
+    a = __shfl_xor_sync(0xffffffffu, high ? v[0] : v[2], 2);
+    b = __shfl_xor_sync(0xffffffffu, high ? v[1] : v[3], 2);
+    if (high) { v[0] = a; v[1] = b; } else { v[2] = a; v[3] = b; }
 }
 
-template <class T, int HD, int RG>
-__global__ void __launch_bounds__(PR_THREADS) paged_rows_kernel(const PagedAttention a, int row_tiles) {
-    extern __shared__ __align__(1024) uint8_t smem[];
-    using L = RowsLayout<HD>;
-    constexpr int KG = 4 / RG, KW = PR_KT / KG, NT = KW / 8, KS = HD / 16, ON = HD / 8, MT = 16 * RG;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, rg = warp % RG, kg = warp / RG;
+template <class T, int HD, int RG, int NR, bool JOIN>
+__global__ void __launch_bounds__(PR_THREADS)
+    paged_rows_kernel(const __grid_constant__ PageMaps maps, const PagedAttention a, const RowsGrid grid) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    using L = RowsLayout<HD, RG>;
+    constexpr int KT = L::KT, MK = KT / 16, KS = HD / 16, MD = HD / 16, WR = 8 * NR, MT = WR * RG;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, rg = warp % RG, team = warp / RG;
 
+    // item = ((sequence, row tile), cached head, split)
+    const uint32_t item = blockIdx.x * (JOIN ? 1 : L::TEAMS) + (JOIN ? 0 : team);
+    if (item >= grid.items) return;
     RowTile t;
-    const int split = int(blockIdx.x % a.splits);
-    {
-        int b = int(blockIdx.x / a.splits);
-        t.m0 = (b % row_tiles) * MT;
-        b /= row_tiles;
-        t.kvh = b % a.cache.kv_heads;
-        t.seq = b / a.cache.kv_heads;
-    }
+    uint32_t split, kvh, rt, seq = grid.row_tiles.divmod(grid.heads.divmod(grid.splits.divmod(item, &split), &kvh), &rt);
+    t.seq = int(seq);
+    t.kvh = int(kvh);
+    t.m0 = int(rt) * MT;
     const SeqInfo q = load_seq(a.batch, t.seq, a.err);
     t.rows = min(MT, q.n * a.group - t.m0);
     if (t.rows <= 0) return;
     t.start = q.start;
-    t.len = q.len;
     t.base = q.len - q.n;
-    const int t_first = t.m0 / a.group, t_last = (t.m0 + t.rows - 1) / a.group;
+    const int t_first = int(grid.group.div(t.m0)), t_last = int(grid.group.div(t.m0 + t.rows - 1));
     t.hi = t.base + t_last + 1;
     t.lo = a.window ? max(0, t.base + t_first - a.window + 1) : 0;
-    // this block's share of the 64-key tiles
-    const int tile0 = t.lo / PR_KT, tiles = (t.hi + PR_KT - 1) / PR_KT - tile0;
-    const int share = (tiles + a.splits - 1) / a.splits;
-    const int first = tile0 + split * share, last = min(first + share, tile0 + tiles);
+    // this item's share of the tiles, and of those this team's
+    const int tile0 = t.lo / KT, tiles = (t.hi + KT - 1) / KT - tile0;
+    const int share = int(grid.splits.div(tiles + a.splits - 1));
+    constexpr int STEP = JOIN ? L::TEAMS : 1;
+    const int first = tile0 + int(split) * share + (JOIN ? team : 0), last = min(tile0 + (int(split) + 1) * share, tile0 + tiles);
 
-    // The two rows of this thread, and their tokens' positions (rows that are not there: a
-    // position before every key).
-    int pos[2];
-    int64_t row_at[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int r = rg * 16 + lane / 4 + 8 * j;
-        const int m = t.m0 + r, tok = m / a.group;
-        pos[j] = r < t.rows ? t.base + tok : -1;
-        row_at[j] = r < t.rows ? (t.start + tok) * a.q.token + (t.kvh * a.group + m - tok * a.group) * a.q.head : -1;
+    uint8_t* ring = smem + team * L::RING;
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::TEAMS * L::RING) + team * L::STAGES;
+    if (rg == 0 && lane == 0) {
+        for (int s = 0; s < L::STAGES; ++s) mbar_init(&full[s], 1);
+        mbar_fence_init();
+        fence_proxy_async();
     }
-    uint32_t qf[KS][4];
+    team_sync<RG>(team);
+
+    // The team's first warp loads: lane p the p-th page that the tile touches.
+    const int slots = 1 << a.cache.page_shift, box = min(slots, KT);
+    const int* table = a.cache.table + int64_t(t.seq) * a.cache.table_stride;
+    auto page_of = [&](int tile) {
+        const int key = tile * KT + lane * box;
+        if (rg != 0 || tile >= last || lane * box >= KT || key + box <= t.lo || key >= t.hi) return -1;
+        const int page = table[key >> a.cache.page_shift];
+        if (page >= 0 && page < a.cache.num_pages) return page;
+        record_error(a.err, kDevBadPage);
+        return a.cache.num_pages;                          // outside the map: zeros
+    };
+    auto load_tile = [&](int tile, int stage, int page) {
+        if (rg != 0) return;
+        const int pieces = __popc(__ballot_sync(0xffffffffu, page >= 0));
+        if (lane == 0) mbar_arrive_expect_tx(&full[stage], pieces * box * HD * 4);
+        __syncwarp();
+        if (page >= 0) {
+            const int slot = (tile * KT + lane * box) & (slots - 1);
+            uint8_t* dst = ring + stage * 2 * L::TILE + lane * box * 128;
 #pragma unroll
-    for (int k = 0; k < KS; ++k)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const T* p = static_cast<const T*>(a.q.data) + row_at[j & 1] + k * 16 + (j >> 1) * 8 + (lane & 3) * 2;
-            qf[k][j] = row_at[j & 1] >= 0 ? *reinterpret_cast<const uint32_t*>(p) : 0u;
+            for (int h = 0; h < HD / 64; ++h) {
+                load_page(dst + h * L::HALF, maps.k, &full[stage], h * 64, slot, t.kvh, page);
+                load_page(dst + L::TILE + h * L::HALF, maps.v, &full[stage], h * 64, slot, t.kvh, page);
+            }
         }
-
-    float o[ON][4];
+        __syncwarp();
+    };
+    int page = page_of(first);
 #pragma unroll
-    for (int n = 0; n < ON; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-    float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
-
-    const uint32_t sbase = smem_u32(smem);
     for (int s = 0; s < L::STAGES - 1; ++s) {
-        if (first + s < last) load_tile<T, HD>(a, t, (first + s) * PR_KT, sbase + s * 2 * L::TILE, sbase + s * 2 * L::TILE + L::TILE);
-        cp_async_commit();
+        if (first + s * STEP < last) load_tile(first + s * STEP, s, page);
+        page = page_of(first + (s + 1) * STEP);
     }
-    int st = 0;
-    for (int tile = first; tile < last; ++tile) {
-        cp_async_wait<L::STAGES - 2>();
-        __syncthreads();
-        {   // the stage read last may be loaded again
-            const int nx = tile + L::STAGES - 1, ns = (st + L::STAGES - 1) % L::STAGES;
-            if (nx < last) load_tile<T, HD>(a, t, nx * PR_KT, sbase + ns * 2 * L::TILE, sbase + ns * 2 * L::TILE + L::TILE);
-            cp_async_commit();
-        }
-        const uint32_t sk = sbase + st * 2 * L::TILE, sv = sk + L::TILE;
-        st = (st + 1) % L::STAGES;
-        const int k0 = tile * PR_KT + kg * KW;
-        float sc[NT][4];
+
+    // Fragments: of a query row this lane holds row lane / 4 (+ 8 n), of a score or weighted value the
+    // rows 2 (lane % 4) + {0, 1} (+ 8 n); pos: the latter's positions (rows that are not there: before
+    // every key).
+    int pos[NR][2];
+    uint32_t qf[KS][NR][2];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+    for (int n = 0; n < NR; ++n) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int r = rg * WR + n * 8 + (lane & 3) * 2 + e;
+            pos[n][e] = r < t.rows ? t.base + int(grid.group.div(t.m0 + r)) : -1;
+        }
+        const int r = rg * WR + n * 8 + lane / 4, m = t.m0 + r, tok = int(grid.group.div(m));
+        const uint32_t* p = reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.q.data) + (t.start + tok) * a.q.token +
+                                                              (t.kvh * a.group + m - tok * a.group) * a.q.head) + (lane & 3);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            qf[k][n][0] = r < t.rows ? p[k * 8] : 0u;
+            qf[k][n][1] = r < t.rows ? p[k * 8 + 4] : 0u;
+        }
+    }
+    float o[MD][NR][4];
+#pragma unroll
+    for (int d = 0; d < MD; ++d)
+#pragma unroll
+        for (int n = 0; n < NR; ++n) o[d][n][0] = o[d][n][1] = o[d][n][2] = o[d][n][3] = 0.f;
+    float mx[NR][2], sum[NR][2];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) { mx[n][0] = mx[n][1] = -INFINITY; sum[n][0] = sum[n][1] = 0.f; }
+
+    int st = 0, phase = 0;
+    bool expired = false;       // after an expired wait the team goes on, without waits, to meet its barriers
+    for (int tile = first; tile < last; tile += STEP) {
+        if (!expired && !mbar_wait(&full[st], phase)) { record_error(a.err, kDevTimeoutAttn); expired = true; }
+        const int k0 = tile * KT;
+        uint8_t* const tk = ring + st * 2 * L::TILE;
+        uint64_t valid = ~0ull;
+        if (a.key_valid) valid = valid_bits(a, t.seq, k0 & ~63) >> (k0 & 63);
+        const bool whole = KT == 64 ? valid == ~0ull : uint32_t(valid) == ~0u;     // every bit is set
+        if (k0 < t.lo || k0 + KT > t.hi || !whole) {
+            // values of keys that no row sees: zeros instead of what stands there
+            for (int r = threadIdx.x % (32 * RG); r < KT; r += 32 * RG) {
+                const int key = k0 + r;
+                if (key >= t.lo && key < t.hi && (((valid >> r) & 1) || (a.self_visible && key >= t.base))) continue;
+#pragma unroll
+                for (int c = 0; c < HD / 8; ++c)
+                    *reinterpret_cast<uint4*>(tk + L::TILE + (c / 8) * L::HALF + r * 128 + (((c + r) & 7) << 4)) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async();                    // before a later load into the stage
+        }
+        team_sync<RG>(team);                        // zeros are written; the stage read last is free
+        {
+            const int nx = tile + (L::STAGES - 1) * STEP, ns = st == 0 ? L::STAGES - 1 : st - 1;
+            if (nx < last) load_tile(nx, ns, page);
+            page = page_of(nx + STEP);
+        }
+        const uint32_t sk = smem_u32(tk), sv = sk + L::TILE;
+        if (++st == L::STAGES) { st = 0; phase ^= 1; }
+        float sc[MK][NR][4];
+#pragma unroll
+        for (int i = 0; i < MK; ++i)
+#pragma unroll
+            for (int n = 0; n < NR; ++n) sc[i][n][0] = sc[i][n][1] = sc[i][n][2] = sc[i][n][3] = 0.f;
+        const uint32_t ka = sk + (lane & 15) * 128, kx = ((lane & 7) ^ (lane >> 4)) << 4;
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
-            for (int n = 0; n < NT; n += 2) {
-                const int r = kg * KW + n * 8 + (lane & 7) + ((lane >> 4) << 3), ch = 2 * k + ((lane >> 3) & 1);
-                uint32_t b[4];
-                ldsm4(sk + r * HD * 2 + ((ch ^ (r & 7)) << 4), b);
-                mma16816<T>(sc[n], qf[k], b[0], b[1]);
-                mma16816<T>(sc[n + 1], qf[k], b[2], b[3]);
+            for (int i = 0; i < MK; ++i) {
+                uint32_t f[4];
+                ldsm4(ka + (k / 4) * L::HALF + i * 16 * 128 + (kx ^ ((k % 4) << 5)), f);
+#pragma unroll
+                for (int n = 0; n < NR; ++n) mma16816<T>(sc[i][n], f, qf[k][n][0], qf[k][n][1]);
             }
         // every row of the tile sees every key of it: no per-key masks
-        const uint64_t valid = valid_bits(a, t.seq, tile * PR_KT);
-        const bool all = tile * PR_KT + PR_KT - 1 <= t.base + t_first && valid == ~0ull &&
-                         (a.window == 0 || tile * PR_KT > t.base + t_last - a.window);
+        const bool all = k0 + KT - 1 <= t.base + t_first && (a.window == 0 || k0 > t.base + t_last - a.window) && whole;
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NR; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                sc[n][e] *= a.scale_log2;
+            for (int e = 0; e < 2; ++e) {
+                // bit 8 j of the row's keys, from this lane's first (lane / 4) on
+                uint64_t see = 0;
                 if (!all) {
-                    const int key = k0 + n * 8 + (lane & 3) * 2 + (e & 1);
-                    if (!sees(a, key, pos[e >> 1], (valid >> (key & 63)) & 1)) sc[n][e] = -INFINITY;
+                    const int p = pos[n][e] - k0;
+                    if (p >= 0) {
+                        see = valid & (p >= 63 ? ~0ull : (2ull << p) - 1);
+                        if (a.window && p >= a.window) see &= p - a.window >= 63 ? 0ull : ~((2ull << (p - a.window)) - 1);
+                        if (a.self_visible && p < 64) see |= 1ull << p;
+                    }
+                    see >>= lane >> 2;
+                }
+#pragma unroll
+                for (int i = 0; i < MK; ++i)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float& x = sc[i][n][2 * h + e];
+                        x *= a.scale_log2;
+                        if (!all && !((see >> (i * 16 + h * 8)) & 1)) x = -INFINITY;
+                    }
+            }
+        // The reference maximum of a row moves only when a score passes it by more than 2^8: then the
+        // sums are scaled down, which most tiles spare.
+        float m[NR][2];
+        bool up = false;
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float x = fmaxf(sc[0][n][e], sc[0][n][2 + e]);
+#pragma unroll
+                for (int i = 1; i < MK; ++i) x = fmaxf(x, fmaxf(sc[i][n][e], sc[i][n][2 + e]));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                m[n][e] = x;
+                up |= x > mx[n][e] + PR_RESCALE;
+            }
+        if (__any_sync(0xffffffffu, up)) {
+#pragma unroll
+            for (int n = 0; n < NR; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    if (m[n][e] > mx[n][e] + PR_RESCALE) {
+                        const float f = exp2_ftz(mx[n][e] - m[n][e]);
+                        mx[n][e] = m[n][e];
+                        sum[n][e] *= f;
+#pragma unroll
+                        for (int d = 0; d < MD; ++d) { o[d][n][e] *= f; o[d][n][2 + e] *= f; }
+                    }
+        }
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float ref = mx[n][e] == -INFINITY ? 0.f : mx[n][e];
+#pragma unroll
+                for (int i = 0; i < MK; ++i) {
+                    sc[i][n][e] = exp2_ftz(sc[i][n][e] - ref);
+                    sc[i][n][2 + e] = exp2_ftz(sc[i][n][2 + e] - ref);
+                    sum[n][e] += sc[i][n][e] + sc[i][n][2 + e];
                 }
             }
+        const uint32_t va = sv + ((lane & 7) + ((lane >> 4) << 3)) * 128, vx = ((lane & 7) ^ ((lane >> 3) & 1)) << 4;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            float m = mx[j];
+        for (int i = 0; i < MK; ++i) {
+            uint32_t p[NR][2];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) m = fmaxf(m, fmaxf(sc[n][2 * j], sc[n][2 * j + 1]));
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-            const float ref = m == -INFINITY ? 0.f : m, f = exp2_ftz(mx[j] - ref);
-            mx[j] = m;
-            float ps = 0.f;
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                sc[n][2 * j] = exp2_ftz(sc[n][2 * j] - ref);
-                sc[n][2 * j + 1] = exp2_ftz(sc[n][2 * j + 1] - ref);
-                ps += sc[n][2 * j] + sc[n][2 * j + 1];
+            for (int n = 0; n < NR; ++n) {
+                p[n][0] = turn8x8(Pair<T>::down(sc[i][n][0], sc[i][n][1]));
+                p[n][1] = turn8x8(Pair<T>::down(sc[i][n][2], sc[i][n][3]));
             }
-            sum[j] = fmaf(sum[j], f, ps);
 #pragma unroll
-            for (int n = 0; n < ON; ++n) { o[n][2 * j] *= f; o[n][2 * j + 1] *= f; }
-        }
+            for (int d = 0; d < MD; ++d) {
+                uint32_t f[4];
+                ldsm4_t(va + (d / 4) * L::HALF + i * 16 * 128 + (vx ^ ((d % 4) << 5)), f);
 #pragma unroll
-        for (int n = 0; n < NT; n += 2) {
-            const uint32_t p[4] = {Pair<T>::down(sc[n][0], sc[n][1]), Pair<T>::down(sc[n][2], sc[n][3]),
-                                   Pair<T>::down(sc[n + 1][0], sc[n + 1][1]), Pair<T>::down(sc[n + 1][2], sc[n + 1][3])};
-#pragma unroll
-            for (int d = 0; d < ON; d += 2) {
-                const int r = kg * KW + n * 8 + (lane & 15), ch = d + (lane >> 4);
-                uint32_t b[4];
-                ldsm4_t(sv + r * HD * 2 + ((ch ^ (r & 7)) << 4), b);
-                mma16816<T>(o[d], p, b[0], b[1]);
-                mma16816<T>(o[d + 1], p, b[2], b[3]);
+                for (int n = 0; n < NR; ++n) mma16816<T>(o[d][n], f, p[n][0], p[n][1]);
             }
         }
     }
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 1);
-        sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 2);
+    for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            sum[n][e] += __shfl_xor_sync(0xffffffffu, sum[n][e], 4);
+            sum[n][e] += __shfl_xor_sync(0xffffffffu, sum[n][e], 8);
+            sum[n][e] += __shfl_xor_sync(0xffffffffu, sum[n][e], 16);
+        }
+    const int64_t part = int64_t(split) * a.batch.tokens * a.q_heads;
+    auto row_of = [&](int r, int64_t* token, int* head) {
+        const int m = t.m0 + r, tok = int(grid.group.div(m));
+        *token = t.start + tok;
+        *head = t.kvh * a.group + m - tok * a.group;
+    };
+    if constexpr (!JOIN) {
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            if (a.splits > 1) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    if (pos[n][e] < 0) continue;
+                    int64_t token;
+                    int head;
+                    row_of(rg * WR + n * 8 + (lane & 3) * 2 + e, &token, &head);
+                    const int64_t at = part + token * a.q_heads + head;
+                    if (lane < 4) a.part_ml[at] = make_float2(mx[n][e], sum[n][e]);
+                    if (mx[n][e] == -INFINITY) continue;
+#pragma unroll
+                    for (int d = 0; d < MD; ++d) {
+                        a.part_o[at * HD + d * 16 + (lane >> 2)] = o[d][n][e];
+                        a.part_o[at * HD + d * 16 + 8 + (lane >> 2)] = o[d][n][2 + e];
+                    }
+                }
+                continue;
+            }
+            // Fragments turn back to rows, 32 columns at a time so that a lane stores 16 bytes; the gate's
+            // 16-bit values turn the other way, so that the product is rounded once.
+            const int r = rg * WR + n * 8 + (lane >> 2);
+            const bool there = r < t.rows;
+            int64_t token;
+            int head;
+            row_of(r, &token, &head);
+            const float inv[2] = {mx[n][0] == -INFINITY ? 0.f : 1.0f / sum[n][0], mx[n][1] == -INFINITY ? 0.f : 1.0f / sum[n][1]};
+            const T* gate = static_cast<const T*>(a.gate.data) + token * a.gate.token + head * a.gate.head;
+            T* out = static_cast<T*>(a.out.data) + token * a.out.token + head * a.out.head;
+#pragma unroll
+            for (int b = 0; b < HD / 8; b += 4) {
+                uint32_t u[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float x = o[(b + i) / 2][n][((b + i) & 1) * 2] * inv[0], y = o[(b + i) / 2][n][((b + i) & 1) * 2 + 1] * inv[1];
+                    if (a.gate.data) {
+                        const uint32_t g = there ? *reinterpret_cast<const uint32_t*>(gate + (b + i) * 8 + (lane & 3) * 2) : 0u;
+                        const float2 gf = Pair<T>::up(turn8x8(g));
+                        x *= gf.x;
+                        y *= gf.y;
+                    }
+                    u[i] = turn8x8(Pair<T>::down(x, y));
+                }
+                quad_transpose(u);
+                if (there) *reinterpret_cast<uint4*>(out + (b + (lane & 3)) * 8) = make_uint4(u[0], u[1], u[2], u[3]);
+            }
+        }
+        return;
     }
-    // Join the key groups through shared memory: per warp 16 rows of HD f32 (four columns of
-    // every row turned by the row, against bank conflicts), maximum and sum.
-    cp_async_wait_all();
+    // Join the teams through shared memory: per warp WR rows of HD f32 (columns of 8 turned by the
+    // row, against bank conflicts), maximum and sum.
     __syncthreads();
-    float* so = reinterpret_cast<float*>(smem) + warp * 16 * HD;
-    float2* sml = reinterpret_cast<float2*>(smem + 4 * 16 * HD * 4);
+    float* so = reinterpret_cast<float*>(smem) + warp * WR * HD;
+    float2* sml = reinterpret_cast<float2*>(smem + 4 * WR * HD * 4);
 #pragma unroll
-    for (int n = 0; n < ON; ++n)
+    for (int n = 0; n < NR; ++n)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int r = lane / 4 + 8 * j, col = n * 8 + (lane & 3) * 2;
-            *reinterpret_cast<float2*>(so + r * HD + (col ^ ((r & 7) << 3))) = make_float2(o[n][2 * j], o[n][2 * j + 1]);
+        for (int e = 0; e < 2; ++e) {
+            const int r = n * 8 + (lane & 3) * 2 + e, x = (lane & 3) << 3;
+#pragma unroll
+            for (int d = 0; d < MD; ++d) {
+                so[r * HD + ((d * 16) ^ x) + (lane >> 2)] = o[d][n][e];
+                so[r * HD + ((d * 16 + 8) ^ x) + (lane >> 2)] = o[d][n][2 + e];
+            }
+            if (lane < 4) sml[warp * WR + r] = make_float2(mx[n][e], sum[n][e]);
         }
-    if ((lane & 3) == 0)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) sml[warp * 16 + lane / 4 + 8 * j] = make_float2(mx[j], sum[j]);
     __syncthreads();
     constexpr int CH = HD / 8;
     for (int i = threadIdx.x; i < t.rows * CH; i += PR_THREADS) {
-        const int r = i / CH, c = i % CH, g = r / 16, rr = r % 16;
+        const int r = i / CH, c = i % CH, g = r / WR, rr = r % WR;
         float m = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < KG; ++k) m = fmaxf(m, sml[(k * RG + g) * 16 + rr].x);
+        for (int k = 0; k < L::TEAMS; ++k) m = fmaxf(m, sml[(k * RG + g) * WR + rr].x);
         float y[8] = {}, l = 0.f;
 #pragma unroll
-        for (int k = 0; k < KG; ++k) {
+        for (int k = 0; k < L::TEAMS; ++k) {
             const int w = k * RG + g;
-            const float2 ml = sml[w * 16 + rr];
+            const float2 ml = sml[w * WR + rr];
             const float f = ml.x == -INFINITY ? 0.f : exp2_ftz(ml.x - m);
             l = fmaf(ml.y, f, l);
-            const float* src = reinterpret_cast<const float*>(smem) + w * 16 * HD + rr * HD + ((c ^ (rr & 7)) << 3);
+            const float* src = reinterpret_cast<const float*>(smem) + w * WR * HD + rr * HD + ((c * 8) ^ (((rr >> 1) & 3) << 3));
 #pragma unroll
             for (int e = 0; e < 8; ++e) y[e] = fmaf(src[e], f, y[e]);
         }
-        const int row = t.m0 + r, tok = row / a.group, head = t.kvh * a.group + row - tok * a.group;
-        const int64_t token = t.start + tok;
+        int64_t token;
+        int head;
+        row_of(r, &token, &head);
         if (a.splits > 1) {
-            const int64_t at = int64_t(split) * a.batch.tokens * a.q_heads + token * a.q_heads + head;
+            const int64_t at = part + token * a.q_heads + head;
             if (c == 0) a.part_ml[at] = make_float2(m, l);
             if (m != -INFINITY) {
                 float4* dst = reinterpret_cast<float4*>(a.part_o + at * HD + c * 8);
@@ -283,87 +484,115 @@ __global__ void __launch_bounds__(PR_THREADS) paged_rows_kernel(const PagedAtten
             }
             continue;
         }
-        const float inv = m == -INFINITY ? 0.f : 1.0f / l;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] *= inv;
-        if (a.gate.data) {
-            float gt[8];
-            unpack8<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(a.gate.data) + token * a.gate.token + head * a.gate.head + c * 8), gt);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] *= gt[e];
-        }
-        *reinterpret_cast<uint4*>(static_cast<T*>(a.out.data) + token * a.out.token + head * a.out.head + c * 8) = pack8<T>(y);
+        store_row<T>(a, token, head, c, y, m == -INFINITY ? 0.f : 1.0f / l);
     }
 }
 
-// Join the splits: item = (new token, query head) of a sequence, HD / 8 threads each.
-template <class T, int HD>
-__global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttention a, int blocks_per_seq) {
-    constexpr int CH = HD / 8, PER = 128 / CH;
+// Join the splits of a (new token, query head) row: HD / 8 threads hold a partial row, G groups of
+// them share the splits out (8 for many splits of few rows, else 2), joined through shared memory.
+template <class T, int HD, int G>
+__global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttention a, const FastDiv chunk, const FastDiv heads) {
+    constexpr int CH = HD / 8, ROWS = 128 / (CH * G);
+    __shared__ float so[ROWS * G][HD];
+    __shared__ float2 sml[ROWS * G];
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int seq = blockIdx.x / blocks_per_seq;
-    const SeqInfo q = load_seq(a.batch, seq, nullptr);
-    const int64_t item = int64_t(blockIdx.x % blocks_per_seq) * PER + threadIdx.x / CH;
-    const int c = threadIdx.x % CH;
-    const int i = int(item / a.q_heads), head = int(item - int64_t(i) * a.q_heads);
-    if (i >= q.n) return;
+    const int slot = threadIdx.x / CH, c = threadIdx.x % CH, g = slot % G;
+    uint32_t i, head;
+    const uint32_t seq = chunk.divmod(heads.divmod(blockIdx.x * ROWS + slot / G, &head), &i);
+    SeqInfo q{};
+    if (seq < uint32_t(a.batch.seqs)) q = load_seq(a.batch, int(seq), nullptr);
+    const bool live = int(i) < q.n;
     const int64_t token = q.start + i, at = token * a.q_heads + head, step = int64_t(a.batch.tokens) * a.q_heads;
-    float m = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[s * step + at].x);
-    float y[8] = {}, l = 0.f;
-    for (int s = 0; s < a.splits; ++s) {
-        const float2 ml = a.part_ml[s * step + at];
-        if (ml.x == -INFINITY) continue;              // saw nothing: no partial row was written
-        const float f = exp2_ftz(ml.x - m);
+    float m = -INFINITY, y[8] = {}, l = 0.f;
+    if (live) {
+#pragma unroll 4
+        for (int s = g; s < a.splits; s += G) {
+            const float2 ml = a.part_ml[s * step + at];
+            if (ml.x == -INFINITY) continue;          // saw nothing: no partial row was written
+            const float4* src = reinterpret_cast<const float4*>(a.part_o + (s * step + at) * HD + c * 8);
+            const float4 u = src[0], w = src[1];
+            const float top = fmaxf(m, ml.x), f = exp2_ftz(ml.x - top), old = exp2_ftz(m - top);
+            m = top;
+            l = fmaf(l, old, ml.y * f);
+            const float p[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = fmaf(y[e], old, p[e] * f);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) so[slot][c * 8 + e] = y[e];
+    if (c == 0) sml[slot] = make_float2(m, l);
+    __syncthreads();
+    if (g != 0 || !live) return;
+    float top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < G; ++k) top = fmaxf(top, sml[slot + k].x);
+    l = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = 0.f;
+#pragma unroll
+    for (int k = 0; k < G; ++k) {
+        const float2 ml = sml[slot + k];
+        if (ml.x == -INFINITY) continue;
+        const float f = exp2_ftz(ml.x - top);
         l = fmaf(ml.y, f, l);
-        const float4* src = reinterpret_cast<const float4*>(a.part_o + (s * step + at) * HD + c * 8);
-        const float4 u = src[0], w = src[1];
-        y[0] = fmaf(u.x, f, y[0]); y[1] = fmaf(u.y, f, y[1]); y[2] = fmaf(u.z, f, y[2]); y[3] = fmaf(u.w, f, y[3]);
-        y[4] = fmaf(w.x, f, y[4]); y[5] = fmaf(w.y, f, y[5]); y[6] = fmaf(w.z, f, y[6]); y[7] = fmaf(w.w, f, y[7]);
-    }
-    const float inv = m == -INFINITY ? 0.f : 1.0f / l;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] *= inv;
-    if (a.gate.data) {
-        float gt[8];
-        unpack8<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(a.gate.data) + token * a.gate.token + head * a.gate.head + c * 8), gt);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] *= gt[e];
+        for (int e = 0; e < 8; ++e) y[e] = fmaf(so[slot + k][c * 8 + e], f, y[e]);
     }
-    *reinterpret_cast<uint4*>(static_cast<T*>(a.out.data) + token * a.out.token + head * a.out.head + c * 8) = pack8<T>(y);
+    store_row<T>(a, token, int(head), c, y, top == -INFINITY ? 0.f : 1.0f / l);
 }
 
-int rows_group(const PagedAttention& a) {
+// Rows of a problem -> warps of a team and their rows: 8, 16, 32 or 64 rows.
+int rows_of_team(const PagedAttention& a) {
     const int64_t rows = int64_t(a.batch.max_chunk) * a.group;
-    return rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
 }
 
-template <class T, int HD, int RG>
+template <class T, int HD, int RG, int NR, bool JOIN>
 cudaError_t launch_rows(const PagedAttention& a, cudaStream_t stream) {
-    using L = RowsLayout<HD>;
+    using L = RowsLayout<HD, RG>;
     static KernelSetup configured;
     int dev = 0;
     cudaGetDevice(&dev);
     unsigned long long key = 0;
     if (configured.needed(dev, &key)) {
-        const cudaError_t e = cudaFuncSetAttribute(paged_rows_kernel<T, HD, RG>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
+        const cudaError_t e = cudaFuncSetAttribute(paged_rows_kernel<T, HD, RG, NR, JOIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
         if (e != cudaSuccess) return e;
         configured.done(dev, key);
     }
-    const int64_t row_tiles = (int64_t(a.batch.max_chunk) * a.group + 16 * RG - 1) / (16 * RG);
-    const int64_t blocks = row_tiles * a.cache.kv_heads * a.batch.seqs;
-    if (blocks * a.splits > INT32_MAX) return cudaErrorInvalidValue;
-    paged_rows_kernel<T, HD, RG><<<unsigned(blocks * a.splits), PR_THREADS, L::SMEM, stream>>>(a, int(row_tiles));
+    constexpr int MT = 8 * NR * RG;
+    const int64_t row_tiles = (int64_t(a.batch.max_chunk) * a.group + MT - 1) / MT;
+    const int64_t items = row_tiles * a.cache.kv_heads * a.batch.seqs * a.splits;
+    if (items > INT32_MAX - 4) return cudaErrorInvalidValue;
+    PageMaps maps;
+    if (!page_maps(&maps, a.cache, std::is_same<T, __nv_bfloat16>::value, L::KT)) return cudaErrorInvalidValue;
+    RowsGrid grid;
+    grid.splits = FastDiv(a.splits);
+    grid.heads = FastDiv(a.cache.kv_heads);
+    grid.row_tiles = FastDiv(uint32_t(row_tiles));
+    grid.group = FastDiv(a.group);
+    grid.items = uint32_t(items);
+    const unsigned blocks = unsigned(JOIN ? items : (items + L::TEAMS - 1) / L::TEAMS);
+    paged_rows_kernel<T, HD, RG, NR, JOIN><<<blocks, PR_THREADS, L::SMEM, stream>>>(maps, a, grid);
     return cudaGetLastError();
 }
-
 template <class T, int HD>
+cudaError_t dispatch_rows(const PagedAttention& a, bool join, cudaStream_t stream) {
+    switch (rows_of_team(a)) {
+        case 8: return join ? launch_rows<T, HD, 1, 1, true>(a, stream) : launch_rows<T, HD, 1, 1, false>(a, stream);
+        case 16: return join ? launch_rows<T, HD, 1, 2, true>(a, stream) : launch_rows<T, HD, 1, 2, false>(a, stream);
+        case 32: return join ? launch_rows<T, HD, 2, 2, true>(a, stream) : launch_rows<T, HD, 2, 2, false>(a, stream);
+        default: return launch_rows<T, HD, 4, 2, false>(a, stream);     // one team
+    }
+}
+
+template <class T, int HD, int G>
 cudaError_t launch_combine(const PagedAttention& a, cudaStream_t stream) {
-    constexpr int PER = 128 / (HD / 8);
-    const int64_t per_seq = (int64_t(a.batch.max_chunk) * a.q_heads + PER - 1) / PER;
-    if (per_seq * a.batch.seqs > INT32_MAX) return cudaErrorInvalidValue;
+    constexpr int ROWS = 128 / (HD / 8 * G);
+    const int64_t rows = int64_t(a.batch.max_chunk) * a.q_heads * a.batch.seqs;
+    if (rows > INT32_MAX - ROWS) return cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(per_seq * a.batch.seqs));
+    cfg.gridDim = dim3(unsigned((rows + ROWS - 1) / ROWS));
     cfg.blockDim = dim3(128);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -371,32 +600,56 @@ cudaError_t launch_combine(const PagedAttention& a, cudaStream_t stream) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, paged_combine_kernel<T, HD>, a, int(per_seq));
+    return cudaLaunchKernelEx(&cfg, paged_combine_kernel<T, HD, G>, a, FastDiv(a.batch.max_chunk), FastDiv(a.q_heads));
 }
 
 template <class T, int HD>
 cudaError_t dispatch(const PagedAttention& a, cudaStream_t stream) {
-    bool taken = false;
-    cudaError_t e = cudaSuccess;
-    if (paged_plan(a).tiles) e = paged_attention_tiles(a, std::is_same<T, __nv_bfloat16>::value, stream, &taken);
-    if (!taken) {
-        const int rg = rows_group(a);
-        e = rg == 1 ? launch_rows<T, HD, 1>(a, stream) : rg == 2 ? launch_rows<T, HD, 2>(a, stream) : launch_rows<T, HD, 4>(a, stream);
-    }
+    const PagedPlan plan = paged_plan(a);
+    const cudaError_t e = plan.tiles ? paged_attention_tiles(a, std::is_same<T, __nv_bfloat16>::value, stream)
+                                     : dispatch_rows<T, HD>(a, plan.join, stream);
     if (e != cudaSuccess || a.splits == 1) return e;
-    return launch_combine<T, HD>(a, stream);
+    return a.splits > 4 ? launch_combine<T, HD, 8>(a, stream) : launch_combine<T, HD, 2>(a, stream);
 }
 
 }  // namespace
 
+// A tensor map over one of the pools, its axes in order of stride (an axis of one entry has none of
+// its own).
+static bool page_map(PageMap* at, const void* base, bool bf16, const PagedCache& c, int64_t page, int64_t head, int64_t slot,
+                     int box_slots) {
+    const int slots = 1 << c.page_shift;
+    struct Axis { int64_t stride, size; int box; int* where; } ax[3] = {{slot, slots, std::min(slots, box_slots), &at->slot},
+                                                                        {head, c.kv_heads, 1, &at->head},
+                                                                        {page, c.num_pages, 1, &at->page}};
+    int64_t top = 0;
+    for (const Axis& x : ax) top = std::max(top, x.size > 1 ? x.stride * x.size : x.stride);
+    for (Axis& x : ax)
+        if (x.size == 1) x.stride = top;
+    std::stable_sort(ax, ax + 3, [](const Axis& x, const Axis& y) { return x.stride < y.stride; });
+    for (int i = 0; i < 3; ++i) *ax[i].where = i + 1;
+    return make_map_4d_16bit(&at->map, base, bf16, c.head_dim, {ax[0].size, ax[1].size, ax[2].size},
+                             {ax[0].stride, ax[1].stride, ax[2].stride}, {ax[0].box, ax[1].box, ax[2].box});
+}
+bool page_maps(PageMaps* m, const PagedCache& c, bool bf16, int box_slots) {
+    return page_map(&m->k, c.k, bf16, c, c.k_page, c.k_head, c.k_slot, box_slots) &&
+           page_map(&m->v, c.v, bf16, c, c.v_page, c.v_head, c.v_slot, box_slots);
+}
+
 PagedPlan paged_plan(const PagedAttention& a) {
     PagedPlan p;
     p.tiles = int64_t(a.batch.max_chunk) * a.group > 64;
-    const int mt = p.tiles ? kPagedTileRows : 16 * rows_group(a), tile = p.tiles ? 128 : 64;
-    const int64_t blocks = (int64_t(a.batch.max_chunk) * a.group + mt - 1) / mt * a.cache.kv_heads * a.batch.seqs;
+    const int64_t rows = int64_t(a.batch.max_chunk) * a.group;
+    const int mt = p.tiles ? kPagedTileRows : rows_of_team(a);
+    const int64_t items = (rows + mt - 1) / mt * a.cache.kv_heads * a.batch.seqs;
     const int keys = a.window ? int(std::min<int64_t>(a.batch.max_length, int64_t(a.window) + a.batch.max_chunk)) : a.batch.max_length;
-    const int64_t want = int64_t(device_sm_count()) * (p.tiles ? 1 : 2);
-    p.splits = int(std::max<int64_t>(1, std::min<int64_t>({(want + blocks - 1) / blocks, (keys + 4 * tile - 1) / (4 * tile), 256})));
+    const int64_t sms = device_sm_count();
+    if (p.tiles) {
+        p.splits = int(std::max<int64_t>(1, std::min<int64_t>({(sms + items - 1) / items, (keys + 511) / 512, 256})));
+    } else {
+        p.join = rows <= 32 && keys > 256;
+        p.splits = int(std::max<int64_t>(1, std::min<int64_t>({items >= sms ? (4 * sms + items - 1) / items : sms / items, (keys + 255) / 256, 256})));
+    }
     p.split_bytes = size_t(a.batch.tokens) * a.q_heads * (size_t(a.cache.head_dim) * 4 + 8);
     return p;
 }

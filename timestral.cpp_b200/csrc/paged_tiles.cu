@@ -18,8 +18,6 @@
 
 namespace tsb {
 
-bool make_map_4d_16bit(CUtensorMap* map, const void* base, bool bf16, int width, const int64_t (&size)[3],
-                       const int64_t (&stride)[3], const int (&box_rows)[3]);
 int device_sm_count();
 
 namespace {
@@ -44,18 +42,6 @@ struct TilesBars {
 };
 static_assert(sizeof(TilesBars) <= 256);
 
-// Which coordinate of a cache's tensor map stands for what (its axes are in order of stride).
-struct PageMap {
-    int slot, head, page;               // 1, 2 or 3
-};
-__device__ __forceinline__ void load_page(void* dst, const CUtensorMap* map, uint64_t* bar, const PageMap& m, int x, int slot,
-                                          int head, int page) {
-    const int c1 = m.slot == 1 ? slot : m.head == 1 ? head : page;
-    const int c2 = m.slot == 2 ? slot : m.head == 2 ? head : page;
-    const int c3 = m.slot == 3 ? slot : m.head == 3 ? head : page;
-    tma_load_4d(dst, map, bar, x, c1, c2, c3);
-}
-
 // Bits [lo, hi] (inclusive, any ints) of the 32-bit word that starts at bit w0.
 __device__ __forceinline__ uint32_t range32(int lo, int hi, int w0) {
     lo = max(lo - w0, 0);
@@ -66,8 +52,7 @@ __device__ __forceinline__ uint32_t range32(int lo, int hi, int w0) {
 
 template <class T, int HD>
 __global__ void __launch_bounds__(PT_THREADS, 1)
-    paged_tiles_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PageMap mk,
-                       const PageMap mv, const PagedAttention a, int row_tiles) {
+    paged_tiles_kernel(const __grid_constant__ PageMaps maps, const PagedAttention a, int row_tiles) {
     using L = TilesLayout<HD>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* qbuf = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -155,7 +140,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                 uint8_t* dst = ring + s * L::SLOT + lane * box * 128;
 #pragma unroll
                 for (int h = 0; h < HD / 64; ++h)
-                    load_page(dst + h * L::HALF, (i & 1) ? &map_v : &map_k, &bars->full[s], (i & 1) ? mv : mk, h * 64, slot, kvh, page);
+                    load_page(dst + h * L::HALF, (i & 1) ? maps.v : maps.k, &bars->full[s], h * 64, slot, kvh, page);
             }
             __syncwarp();
         }
@@ -370,36 +355,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     if (warp == 8) tmem_dealloc(tbase, PT_TMEM);
 }
 
-// A tensor map over one of the pools, its axes in order of stride (an axis of one entry has none of
-// its own), in boxes of `box` slots.
-bool page_map(CUtensorMap* map, PageMap* at, const void* base, bool bf16, const PagedCache& c, int64_t page, int64_t head,
-              int64_t slot) {
-    const int slots = 1 << c.page_shift;
-    struct Axis { int64_t stride, size; int box; int* where; } ax[3] = {{slot, slots, std::min(slots, PT_KT), &at->slot},
-                                                                        {head, c.kv_heads, 1, &at->head},
-                                                                        {page, c.num_pages, 1, &at->page}};
-    int64_t top = 0;
-    for (const Axis& x : ax) top = std::max(top, x.size > 1 ? x.stride * x.size : x.stride);
-    for (Axis& x : ax)
-        if (x.size == 1) x.stride = top;
-    std::stable_sort(ax, ax + 3, [](const Axis& x, const Axis& y) { return x.stride < y.stride; });
-    for (int i = 0; i < 3; ++i) *ax[i].where = i + 1;
-    return make_map_4d_16bit(map, base, bf16, c.head_dim, {ax[0].size, ax[1].size, ax[2].size},
-                             {ax[0].stride, ax[1].stride, ax[2].stride}, {ax[0].box, ax[1].box, ax[2].box});
-}
-
 template <class T, int HD>
-cudaError_t launch_tiles(const PagedAttention& a, cudaStream_t stream, bool* taken) {
+cudaError_t launch_tiles(const PagedAttention& a, cudaStream_t stream) {
     using L = TilesLayout<HD>;
-    constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
-    *taken = false;
+    const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
     const PagedCache& c = a.cache;
-    CUtensorMap map_k, map_v;
-    PageMap mk, mv;
-    if (!page_map(&map_k, &mk, c.k, bf16, c, c.k_page, c.k_head, c.k_slot) ||
-        !page_map(&map_v, &mv, c.v, bf16, c, c.v_page, c.v_head, c.v_slot))
-        return cudaSuccess;
-    *taken = true;
+    PageMaps maps;
+    if (!page_maps(&maps, c, bf16, PT_KT)) return cudaErrorInvalidValue;
     static KernelSetup configured;
     int dev = 0;
     cudaGetDevice(&dev);
@@ -412,16 +374,16 @@ cudaError_t launch_tiles(const PagedAttention& a, cudaStream_t stream, bool* tak
     const int64_t row_tiles = (int64_t(a.batch.max_chunk) * a.group + kPagedTileRows - 1) / kPagedTileRows;
     const int64_t blocks = row_tiles * c.kv_heads * a.batch.seqs * a.splits;
     if (blocks > INT32_MAX) return cudaErrorInvalidValue;
-    paged_tiles_kernel<T, HD><<<unsigned(blocks), PT_THREADS, L::SMEM, stream>>>(map_k, map_v, mk, mv, a, int(row_tiles));
+    paged_tiles_kernel<T, HD><<<unsigned(blocks), PT_THREADS, L::SMEM, stream>>>(maps, a, int(row_tiles));
     return cudaGetLastError();
 }
 
 }  // namespace
 
-cudaError_t paged_attention_tiles(const PagedAttention& a, bool bf16, cudaStream_t stream, bool* taken) {
+cudaError_t paged_attention_tiles(const PagedAttention& a, bool bf16, cudaStream_t stream) {
     if (a.cache.head_dim == 64)
-        return bf16 ? launch_tiles<__nv_bfloat16, 64>(a, stream, taken) : launch_tiles<__half, 64>(a, stream, taken);
-    return bf16 ? launch_tiles<__nv_bfloat16, 128>(a, stream, taken) : launch_tiles<__half, 128>(a, stream, taken);
+        return bf16 ? launch_tiles<__nv_bfloat16, 64>(a, stream) : launch_tiles<__half, 64>(a, stream);
+    return bf16 ? launch_tiles<__nv_bfloat16, 128>(a, stream) : launch_tiles<__half, 128>(a, stream);
 }
 
 }  // namespace tsb

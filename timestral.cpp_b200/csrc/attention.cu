@@ -794,16 +794,6 @@ __device__ __forceinline__ AlProblem al_problem(const MaskMeta& mm, int p, int R
     return a;
 }
 
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-
 // Walks the key (or value) tiles of this CTA's problems in order.
 struct TileCursor {
     int p = 0, i = 0, j = 0, n = 0, g = 0, rh = 0;

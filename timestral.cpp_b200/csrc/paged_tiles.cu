@@ -3,11 +3,13 @@
 // A block owns 256 rows (token, query head of the group) of one (sequence, cached head) as two
 // tiles of 128 and streams the keys and values that they see in tiles of 128, so that a tile in
 // shared memory serves both row tiles. Warps 0-3 and 4-7 hold the two row tiles, a thread a row
-// (TMEM lane); warp 8 issues the MMAs, warp 9 the TMA loads, one per page that the tile touches.
+// (TMEM lane); warp 8 issues the MMAs, warp 9 the TMA loads, one per page that a tile touches.
 // TMEM (512 columns): the scores S of each row tile (128 columns), which its f16 probabilities
 // overwrite (two keys a column), and its weighted values O. The MMAs of one row tile run while
 // the other's softmax does: per key tile, in the order of issue and so of execution,
 //   O0 += P0 V_j, S0 = Q0 K_{j+1}, O1 += P1 V_j, S1 = Q1 K_{j+1}.
+// (A warp for each row tile's MMAs let them mix, so that both softmaxes waited and ran together:
+// 1.17 -> 1.36 ms for 2048 tokens of 32 heads over 34,816 keys.)
 // A commit covers every earlier MMA, so a full S_{j+1} also says that O holds tile j: the softmax
 // may rescale it. It does so only when a row's maximum passes its reference by more than 2^8
 // (probabilities then lie in (0, 256]).
@@ -22,9 +24,15 @@ int device_sm_count();
 
 namespace {
 
-constexpr int PT_THREADS = 320;
+constexpr int PT_THREADS = 384;         // two softmax warpgroups; MMA, TMA and two idle warps
+// The softmax warpgroups take registers from the third: 2 * 128 * 216 + 128 * 72 = 384 * 168, what
+// the block is launched with.
+constexpr int PT_LAUNCH_REGS = 168, PT_SOFTMAX_REGS = 216, PT_OTHER_REGS = 72;
+static_assert(256 * PT_SOFTMAX_REGS + 128 * PT_OTHER_REGS <= PT_THREADS * PT_LAUNCH_REGS);
 constexpr int PT_KT = 128;
 constexpr uint32_t PT_TMEM = 512, PT_O_COL = 256;
+// Of every PT_POLY_OF pairs of probabilities so many come from exp2_poly.
+constexpr int PT_POLY_OF = 8, PT_POLY_64 = 0, PT_POLY_128 = 0;
 constexpr float PT_RESCALE = 8.f;       // log2 of the largest probability kept unscaled
 
 template <int HD>
@@ -36,11 +44,38 @@ struct TilesLayout {
 };
 
 struct TilesBars {
-    uint64_t full[8], empty[8], q_ready[2], s_full[2], p_ready[2], o_full[2];
+    uint64_t full[8], empty[8], q_ready[2], s_full[2], p_ready[2][2], o_full[2];
     uint32_t tmem;
     int abort;
 };
 static_assert(sizeof(TilesBars) <= 256);
+
+// Bounded waits of this kernel's roles. No suspend-time hint: a warp that sleeps on one wakes some
+// hundred cycles late, which stands between every two steps here (1.19 -> 1.09 ms for 2048 tokens of
+// 32 heads over 34,816 keys).
+__device__ __forceinline__ bool try_wait(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool role_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* err) {
+    if (try_wait(bar, parity)) return true;
+    const long long start = clock64();
+    while (true) {
+        if (try_wait(bar, parity)) return true;
+        if (*abort) return false;
+        if (clock64() - start > kWaitCycles) { *abort = 1; record_error(err, kDevTimeoutAttn); return false; }
+    }
+}
+// Every lane waits; the warp goes on together.
+__device__ __forceinline__ bool role_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort, int* err) {
+    const bool ok = role_wait(bar, parity, abort, err);
+    return __all_sync(0xffffffffu, ok);
+}
 
 // Bits [lo, hi] (inclusive, any ints) of the 32-bit word that starts at bit w0.
 __device__ __forceinline__ uint32_t range32(int lo, int hi, int w0) {
@@ -48,6 +83,51 @@ __device__ __forceinline__ uint32_t range32(int lo, int hi, int w0) {
     hi = min(hi - w0, 31);
     if (lo > hi) return 0u;
     return (0xffffffffu >> (31 - hi)) & (0xffffffffu << lo);
+}
+
+__device__ __forceinline__ uint64_t desc_of(uint32_t lo, uint32_t hi) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
+    return d;
+}
+// Two f32 values in a register pair, for the instructions that work on both at once.
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 f2(float a, float b) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void f2_split(F2 x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+__device__ __forceinline__ F2 f2_add(F2 a, F2 b) {
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+// 2^x of two values at most 2^7, on the FMA pipe: x = n + f with |f| <= 1/2 (n read off the low bits of
+// x + 1.5 * 2^23), 2^f by a polynomial of degree 4 (least largest relative error on the interval:
+// 2.6e-6, far below a probability's rounding to 16 bits), n added to its exponent. Values below -126 are
+// taken as -126: a probability that rounds to nothing. The exponential unit does four a cycle and
+// scheduler, which alone would take as long as the MMAs at head_dim 128 and twice as long at 64.
+__device__ __forceinline__ void exp2_poly(F2 x, float& r0, float& r1) {
+    float a, b;
+    f2_split(x, a, b);
+    x = f2(fmaxf(a, -126.f), fmaxf(b, -126.f));
+    const F2 magic = f2(12582912.f, 12582912.f), minus = f2(-12582912.f, -12582912.f), neg = f2(-1.f, -1.f);
+    const F2 t = f2_add(x, magic), f = f2_fma(f2_add(t, minus), neg, x);
+    F2 p = f2_fma(f2(0.009570100344717503f, 0.009570100344717503f), f, f2(0.05591786280274391f, 0.05591786280274391f));
+    p = f2_fma(p, f, f2(0.240247443318367f, 0.240247443318367f));
+    p = f2_fma(p, f, f2(0.6931217908859253f, 0.6931217908859253f));
+    p = f2_fma(p, f, f2(0.9999992847442627f, 0.9999992847442627f));
+    float t0, t1, p0, p1;
+    f2_split(t, t0, t1);
+    f2_split(p, p0, p1);
+    r0 = __int_as_float(__float_as_int(p0) + (__float_as_int(t0) << 23));
+    r1 = __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23));
 }
 
 template <class T, int HD>
@@ -102,7 +182,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
         for (int s = 0; s < L::STAGES; ++s) { mbar_init(&bars->full[s], 1); mbar_init(&bars->empty[s], 1); }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bars->q_ready[i], 4); mbar_init(&bars->s_full[i], 1);
-            mbar_init(&bars->p_ready[i], 4); mbar_init(&bars->o_full[i], 1);
+            mbar_init(&bars->p_ready[i][0], 4); mbar_init(&bars->p_ready[i][1], 4); mbar_init(&bars->o_full[i], 1);
         }
         bars->abort = 0;
         mbar_fence_init();
@@ -114,91 +194,102 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     tc_fence_after();
     const uint32_t tbase = bars->tmem;
 
-    if (warp == 9) {
-        // TMA producer: K_0, V_0, K_1, V_1, ... through one ring; lane p loads page piece p of a tile.
-        const int slots = 1 << a.cache.page_shift, box = min(slots, PT_KT);
-        const int* table = a.cache.table + int64_t(seq) * a.cache.table_stride;
-        const int key0 = first * PT_KT + lane * box;
-        auto page_of = [&](int j) {
-            const int key = key0 + j * PT_KT;
-            if (lane * box >= PT_KT || j >= nt || key + box <= lo || key >= hi) return -1;
-            const int page = table[key >> a.cache.page_shift];
-            if (page >= 0 && page < a.cache.num_pages) return page;
-            record_error(a.err, kDevBadPage);
-            return a.cache.num_pages;                              // outside the map: zeros
-        };
-        int next = page_of(0), page = -1;
-        for (int i = 0; i < 2 * nt; ++i) {
-            const int j = i >> 1, s = i % L::STAGES;
-            if ((i & 1) == 0) { page = next; next = page_of(j + 1); }
-            if (i >= L::STAGES && !warp_wait(&bars->empty[s], ((i / L::STAGES) - 1) & 1, abort, a.err)) break;
-            const int pieces = __popc(__ballot_sync(0xffffffffu, page >= 0));
-            if (lane == 0) mbar_arrive_expect_tx(&bars->full[s], pieces * box * HD * 2);
-            __syncwarp();
-            if (page >= 0) {
-                const int slot = (key0 + j * PT_KT) & (slots - 1);
-                uint8_t* dst = ring + s * L::SLOT + lane * box * 128;
-#pragma unroll
-                for (int h = 0; h < HD / 64; ++h)
-                    load_page(dst + h * L::HALF, (i & 1) ? maps.v : maps.k, &bars->full[s], h * 64, slot, kvh, page);
-            }
-            __syncwarp();
-        }
-    } else if (warp == 8) {
-        if (lane == 0) {
-            constexpr uint32_t bf = std::is_same<T, __nv_bfloat16>::value ? kIdescBf16 : 0u;
-            const uint32_t id_qk = idesc_f16(128, PT_KT) | bf, id_pv = idesc_f16_bmn(128, HD) | bf;
-            auto scores = [&](int gg, int j) {                      // S_gg = Q_gg K_j
-                const uint64_t dq = smem_desc_sw128(smem_u32(qbuf + gg * L::SLOT));
-                const uint64_t dk = smem_desc_sw128(smem_u32(ring + (2 * j) % L::STAGES * L::SLOT));
-#pragma unroll
-                for (int k = 0; k < HD / 16; ++k) {
-                    const uint64_t off = uint64_t((k / 4) * (L::HALF >> 4) + (k % 4) * 2);
-                    mma_f16(tbase + gg * 128, dq + off, dk + off, id_qk, k > 0);
-                }
-                mma_commit(&bars->s_full[gg]);
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PT_OTHER_REGS));
+        if (warp == 9) {
+            // TMA producer: K_0, V_0, K_1, V_1, ... through one ring; lane p loads page piece p of a tile.
+            const int slots = 1 << a.cache.page_shift, box = min(slots, PT_KT);
+            const int* table = a.cache.table + int64_t(seq) * a.cache.table_stride;
+            const int key0 = first * PT_KT + lane * box;
+            auto page_of = [&](int j) {
+                const int key = key0 + j * PT_KT;
+                if (lane * box >= PT_KT || j >= nt || key + box <= lo || key >= hi) return -1;
+                const int page = table[key >> a.cache.page_shift];
+                if (page >= 0 && page < a.cache.num_pages) return page;
+                record_error(a.err, kDevBadPage);
+                return a.cache.num_pages;                              // outside the map: zeros
             };
-            auto full = [&](int i) { return at_wait(&bars->full[i % L::STAGES], (i / L::STAGES) & 1, abort, a.err); };
-            auto release = [&](int i) { mma_commit(&bars->empty[i % L::STAGES]); };
-            bool ok = full(0);
+            int next = page_of(0), page = -1;
+            for (int i = 0; i < 2 * nt; ++i) {
+                const int j = i >> 1, s = i % L::STAGES;
+                if ((i & 1) == 0) { page = next; next = page_of(j + 1); }
+                if (i >= L::STAGES && !role_wait_warp(&bars->empty[s], ((i / L::STAGES) - 1) & 1, abort, a.err)) break;
+                const int pieces = __popc(__ballot_sync(0xffffffffu, page >= 0));
+                if (lane == 0) mbar_arrive_expect_tx(&bars->full[s], pieces * box * HD * 2);
+                __syncwarp();
+                if (page >= 0) {
+                    const int slot = (key0 + j * PT_KT) & (slots - 1);
+                    uint8_t* dst = ring + s * L::SLOT + lane * box * 128;
 #pragma unroll
-            for (int gg = 0; gg < 2; ++gg)
-                if (ok && ng[gg] > 0) {
-                    ok = at_wait(&bars->q_ready[gg], 0, abort, a.err);
-                    tc_fence_after();
-                    if (ok) scores(gg, 0);
+                    for (int h = 0; h < HD / 64; ++h)
+                        load_page(dst + h * L::HALF, (i & 1) ? maps.v : maps.k, &bars->full[s], h * 64, slot, kvh, page);
                 }
-            if (ok) release(0);
-            for (int j = 0; j < nt && ok; ++j) {
-                ok = full(2 * j + 1);
-                const uint32_t sv = smem_u32(ring + (2 * j + 1) % L::STAGES * L::SLOT);
-                bool have_k = false;
-#pragma unroll
-                for (int gg = 0; gg < 2; ++gg) {
-                    if (ok && j < ng[gg]) {
-                        ok = at_wait(&bars->p_ready[gg], j & 1, abort, a.err);
-                        tc_fence_after();
-                        if (ok) {
-#pragma unroll
-                            for (int kk = 0; kk < PT_KT / 16; ++kk)
-                                mma_f16_ts(tbase + PT_O_COL + gg * 128, tbase + gg * 128 + kk * 8,
-                                           smem_desc_sw128_mn(sv + kk * 16 * 128, L::HALF), id_pv, j > 0 || kk > 0);
-                            if (j + 1 == ng[gg]) mma_commit(&bars->o_full[gg]);
-                        }
-                    }
-                    if (ok && gg == 1) release(2 * j + 1);
-                    if (ok && j + 1 < ng[gg]) {
-                        if (!have_k) ok = full(2 * j + 2);
-                        have_k = true;
-                        tc_fence_after();
-                        if (ok) scores(gg, j + 1);
-                    }
-                }
-                if (ok && j + 1 < nt) release(2 * j + 2);
+                __syncwarp();
             }
+        } else if (warp == 8) {
+            if (lane == 0) {
+                // Few instructions between the MMAs, which they would hold up: descriptors differ from the ring
+                // slot's in their low word alone, by constants.
+                constexpr uint32_t bf = std::is_same<T, __nv_bfloat16>::value ? kIdescBf16 : 0u;
+                const uint32_t id_qk = idesc_f16(128, PT_KT) | bf, id_pv = idesc_f16_bmn(128, HD) | bf;
+                const uint64_t dq = smem_desc_sw128(smem_u32(qbuf)), dr = smem_desc_sw128(smem_u32(ring));
+                const uint64_t dv = smem_desc_sw128_mn(smem_u32(ring), L::HALF);
+                const uint32_t hi = uint32_t(dq >> 32), hi_v = uint32_t(dv >> 32), lo_q = uint32_t(dq), lo_r = uint32_t(dr), lo_v = uint32_t(dv);
+                constexpr uint32_t SLOT16 = L::SLOT >> 4;
+                int slot = 0, phase = 0;                                // of the next tile in the ring
+                auto full = [&]() { return role_wait(&bars->full[slot], phase, abort, a.err); };
+                auto next = [&]() { if (++slot == L::STAGES) { slot = 0; phase ^= 1; } };
+                auto scores = [&](int gg) {                             // S_gg = Q_gg K of the ring's next tile
+                    const uint32_t q = lo_q + gg * SLOT16, k = lo_r + slot * SLOT16;
+#pragma unroll
+                    for (int i = 0; i < HD / 16; ++i) {
+                        const uint32_t off = (i / 4) * (L::HALF >> 4) + (i % 4) * 2;
+                        mma_f16(tbase + gg * 128, desc_of(q + off, hi), desc_of(k + off, hi), id_qk, i > 0);
+                    }
+                    mma_commit(&bars->s_full[gg]);
+                };
+                bool ok = full();
+#pragma unroll
+                for (int gg = 0; gg < 2; ++gg)
+                    if (ok && ng[gg] > 0) {
+                        ok = role_wait(&bars->q_ready[gg], 0, abort, a.err);
+                        tc_fence_after();
+                        if (ok) scores(gg);
+                    }
+                if (ok) mma_commit(&bars->empty[0]);
+                next();
+                for (int j = 0; j < nt && ok; ++j) {
+                    ok = full();
+                    const int vslot = slot;
+                    const uint32_t v = lo_v + slot * SLOT16;
+                    next();
+                    if (ok && j + 1 < nt) ok = full();
+#pragma unroll
+                    for (int gg = 0; gg < 2; ++gg) {
+                        if (ok && j < ng[gg]) {
+                            // the first half of the probabilities is multiplied while the second is made
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                if (ok) ok = role_wait(&bars->p_ready[gg][h], j & 1, abort, a.err);
+                                tc_fence_after();
+                                if (!ok) break;
+#pragma unroll
+                                for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
+                                    mma_f16_ts(tbase + PT_O_COL + gg * 128, tbase + gg * 128 + kk * 8, desc_of(v + kk * 128, hi_v), id_pv,
+                                               j > 0 || kk > 0);
+                            }
+                            if (ok && j + 1 < ng[gg]) scores(gg);
+                            if (ok && j + 1 == ng[gg]) mma_commit(&bars->o_full[gg]);
+                        }
+                        if (ok && gg == 1) mma_commit(&bars->empty[vslot]);
+                    }
+                    if (ok && j + 1 < nt) { mma_commit(&bars->empty[slot]); next(); }
+                }
+            }
+            __syncwarp();
         }
-        __syncwarp();
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PT_SOFTMAX_REGS));
         // Softmax of row `row`, a thread of TMEM lane t.
         const int ngg = g ? ng[1] : ng[0];
         const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
@@ -234,7 +325,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             if (dead_keys && g == (j < ng[0] ? 0 : 1)) {
                 // values of keys that no row of the block sees: zeros instead of what stands there
                 const int i = 2 * j + 1;
-                if (!(ok = warp_wait(&bars->full[i % L::STAGES], (i / L::STAGES) & 1, abort, a.err))) break;
+                if (!(ok = role_wait_warp(&bars->full[i % L::STAGES], (i / L::STAGES) & 1, abort, a.err))) break;
                 const int key = k0 + t;
                 const bool valid = ((t < 64 ? v01 >> t : v23 >> (t - 64)) & 1) || (a.self_visible && key >= base);
                 if (key < lo || key >= hi || !valid) {
@@ -246,28 +337,28 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                 }
                 fence_proxy_async();
             }
-            if (!(ok = warp_wait(&bars->s_full[g], j & 1, abort, a.err))) break;
+            if (!(ok = role_wait_warp(&bars->s_full[g], j & 1, abort, a.err))) break;
             tc_fence_after();
+            // a quarter of the scores is loaded while the maximum of the one before is taken
             uint32_t s[4][32];
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            const uint32_t vw[4] = {uint32_t(v01), uint32_t(v01 >> 32), uint32_t(v23), uint32_t(v23 >> 32)};
+            tmem_ld32(ts, s[0]);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, s[c]);
-            tmem_ld_wait();
-            if (!plain) {
-                const uint32_t vw[4] = {uint32_t(v01), uint32_t(v01 >> 32), uint32_t(v23), uint32_t(v23 >> 32)};
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
+            for (int c = 0; c < 4; ++c) {
+                tmem_ld_wait32(s[c]);
+                if (c < 3) tmem_ld32(ts + (c + 1) * 32, s[c + 1]);
+                if (!plain) {
                     const int w0 = k0 + c * 32;
                     const uint32_t see = (vw[c] & range32(from, pos, w0)) | (a.self_visible ? range32(pos, pos, w0) : 0u);
 #pragma unroll
                     for (int e = 0; e < 32; ++e)
                         if (!((see >> e) & 1u)) s[c][e] = __float_as_uint(-INFINITY);
                 }
+#pragma unroll
+                for (int e = 0; e < 32; e += 2)
+                    mx[(e / 2) & 3] = fmaxf(fmaxf(mx[(e / 2) & 3], __uint_as_float(s[c][e])), __uint_as_float(s[c][e + 1]));
             }
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int e = 0; e < 32; e += 2)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) mx[c] = fmaxf(fmaxf(mx[c], __uint_as_float(s[c][e])), __uint_as_float(s[c][e + 1]));
             const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
             const bool need = mref != -INFINITY && mt > mref + PT_RESCALE;
             float factor = 1.f;
@@ -285,27 +376,38 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                 }
             }
             const float off = mref == -INFINITY ? 0.f : mref;
-            float ps[4] = {0.f, 0.f, 0.f, 0.f};
+            const F2 scale2 = f2(scale, scale), off2 = f2(-off, -off);
+            F2 ps[4] = {f2(0.f, 0.f), f2(0.f, 0.f), f2(0.f, 0.f), f2(0.f, 0.f)};
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 uint32_t pk[32];
 #pragma unroll
                 for (int e = 0; e < 32; ++e) {
                     const int c = half * 2 + e / 16, k = (e % 16) * 2;
-                    const float e0 = exp2_ftz(__fmaf_rn(__uint_as_float(s[c][k]), scale, -off));
-                    const float e1 = exp2_ftz(__fmaf_rn(__uint_as_float(s[c][k + 1]), scale, -off));
-                    ps[e & 3] += e0 + e1;
+                    const F2 x = f2_fma(f2(__uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1])), scale2, off2);
+                    float e0, e1;
+                    if (e % PT_POLY_OF < (HD == 64 ? PT_POLY_64 : PT_POLY_128)) {
+                        exp2_poly(x, e0, e1);
+                    } else {
+                        f2_split(x, e0, e1);
+                        e0 = exp2_ftz(e0);
+                        e1 = exp2_ftz(e1);
+                    }
+                    ps[e & 3] = f2_add(ps[e & 3], f2(e0, e1));
                     pk[e] = Pair<T>::down(e0, e1);
                 }
                 tmem_st32(ts + half * 32, pk);
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars->p_ready[g][half]);
             }
-            sum += (ps[0] + ps[1]) + (ps[2] + ps[3]);
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bars->p_ready[g]);
+            const F2 both = f2_add(f2_add(ps[0], ps[1]), f2_add(ps[2], ps[3]));
+            float s0, s1;
+            f2_split(both, s0, s1);
+            sum += s0 + s1;
         }
-        if (ok && ngg > 0) ok = warp_wait(&bars->o_full[g], 0, abort, a.err);
+        if (ok && ngg > 0) ok = role_wait_warp(&bars->o_full[g], 0, abort, a.err);
         if (ok) {
             tc_fence_after();
             const bool none = ngg == 0;
@@ -369,6 +471,11 @@ cudaError_t launch_tiles(const PagedAttention& a, cudaStream_t stream) {
     if (configured.needed(dev, &key)) {
         const cudaError_t e = cudaFuncSetAttribute(paged_tiles_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
         if (e != cudaSuccess) return e;
+        // the register shares above must not exceed what the block is launched with
+        cudaFuncAttributes fa;
+        const cudaError_t f = cudaFuncGetAttributes(&fa, paged_tiles_kernel<T, HD>);
+        if (f != cudaSuccess) return f;
+        if (fa.numRegs < PT_LAUNCH_REGS) return cudaErrorLaunchOutOfResources;
         configured.done(dev, key);
     }
     const int64_t row_tiles = (int64_t(a.batch.max_chunk) * a.group + kPagedTileRows - 1) / kPagedTileRows;

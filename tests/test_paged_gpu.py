@@ -311,8 +311,9 @@ def test_attention_strides_scale_and_output_in_place(new, lengths, order):
 def test_attention_splits_as_far_as_the_workspace_goes(new, lengths):
     b = ref.Batch(new, lengths, 4, 2, 128, 64, torch.float16)
     want, tol = ref.attention(b)
-    one = b.tokens * b.qh * (128 * 4 + 8)
-    for size in (0, one - 4, 2 * one, 3 * one + 8, "full"):
+    full = tb.paged_attention_workspace(*handles(b), b.tokens, b.qh)
+    assert full > 0
+    for size in (0, 4, full // 4, full // 2, full - 4, "full"):
         a = attend(b, workspace=size)
         ref.within(a, want, tol)
         assert torch.equal(a, attend(b, workspace=size))          # the same bits every time

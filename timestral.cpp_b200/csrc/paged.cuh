@@ -71,17 +71,63 @@ struct PagedAttention {
     const uint32_t* key_valid = nullptr;
     int64_t key_valid_stride = 0;
     int key_valid_positions = 0;
-    int splits = 1;
-    float* part_o = nullptr;            // [splits][tokens * q_heads][head_dim], unnormalised
-    float2* part_ml = nullptr;          // [splits][tokens * q_heads]: reference maximum (log2 units), sum
+    int splits = 1;                     // of the items behind the grid's first `whole`
+    float* part_o = nullptr;            // [items - whole][splits][tile_rows][head_dim], unnormalised
+    float2* part_ml = nullptr;          // the same rows: reference maximum (log2 units), sum
     int* err = nullptr;
 };
+
+// Division by a number known at launch: n / d for n < 2^31 as the high word of a product.
+struct FastDiv {
+    uint32_t d = 1, mul = 0, shift = 0;
+    FastDiv() = default;
+    explicit FastDiv(uint32_t divisor) : d(divisor) {
+        if (d == 1) return;
+        while ((1ull << shift) < d) ++shift;                       // mul = ceil(2^(31 + shift) / d) < 2^32
+        mul = uint32_t(((1ull << (31 + shift)) + d - 1) / d);
+        --shift;
+    }
+    __device__ __forceinline__ uint32_t div(uint32_t n) const { return d == 1 ? n : __umulhi(n, mul) >> shift; }
+    __device__ __forceinline__ uint32_t divmod(uint32_t n, uint32_t* rest) const {
+        const uint32_t x = div(n);
+        *rest = n - x * d;
+        return x;
+    }
+};
+
+// The work of a call: an item is a tile of rows of one (sequence, cached head), those with the last
+// rows (which see most keys) first. The first `whole` items are one unit each, the others a unit for
+// each split of their keys.
+struct PagedGrid {
+    FastDiv splits, heads, seqs, group;
+    uint32_t items = 0, whole = 0, units = 0, row_tiles = 0;
+};
+struct PagedItem {
+    int row_tile, kvh, seq;
+};
+__device__ __forceinline__ PagedItem item_of(const PagedGrid& g, uint32_t item) {
+    uint32_t kvh, seq;
+    const uint32_t back = g.seqs.divmod(g.heads.divmod(item, &kvh), &seq);
+    return {int(g.row_tiles - 1 - back), int(kvh), int(seq)};
+}
+// A unit's item, its split, and into how many its item is split.
+__device__ __forceinline__ uint32_t unit_of(const PagedGrid& g, uint32_t unit, uint32_t* split, int* splits) {
+    if (unit < g.whole) {
+        *split = 0;
+        *splits = 1;
+        return unit;
+    }
+    *splits = int(g.splits.d);
+    return g.whole + g.splits.divmod(unit - g.whole, split);
+}
 
 // How a call of paged_attention runs: chosen from sizes alone, so that the workspace query and
 // the call agree. splits is what it would like without a bound on the workspace.
 struct PagedPlan {
     bool tiles = false;                 // paged_attention_tiles, else paged_attention_rows
     bool join = false;                  // rows: a block's teams share one problem
+    int tile_rows = 0;
+    int64_t row_tiles = 0, items = 0, whole = 0;
     int splits = 1;
     size_t split_bytes = 0;             // workspace bytes of one split
 };
@@ -92,7 +138,7 @@ cudaError_t norm_rope(const NormRope& a, bool bf16, cudaStream_t stream);
 cudaError_t paged_append(const PagedAppend& a, bool bf16, cudaStream_t stream);
 cudaError_t paged_attention(const PagedAttention& a, bool bf16, cudaStream_t stream);
 // The kernel for many rows (paged_tiles.cu).
-cudaError_t paged_attention_tiles(const PagedAttention& a, bool bf16, cudaStream_t stream);
+cudaError_t paged_attention_tiles(const PagedAttention& a, const PagedGrid& grid, bool bf16, cudaStream_t stream);
 constexpr int kPagedTileRows = 256;     // its rows per block
 
 // A tensor map over one of the cache's pools: 64 values by up to box_slots slots of one head and

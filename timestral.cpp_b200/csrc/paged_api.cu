@@ -275,11 +275,11 @@ extern "C" TIMESTRAL_API int tsb_paged_attention(const tsb_paged_attention_args*
         return r.report();
     tsb::PagedAttention p = attention_of(*a);
     const tsb::PagedPlan plan = tsb::paged_plan(p);
-    const size_t held = a->workspace ? a->workspace_bytes / plan.split_bytes : 0;
+    const size_t held = a->workspace && plan.split_bytes ? a->workspace_bytes / plan.split_bytes : 0;
     p.splits = held < 2 ? 1 : int(held < size_t(plan.splits) ? held : size_t(plan.splits));
     if (p.splits > 1) {
-        // weighted values [splits][tokens * q_heads][head_dim], then their (maximum, sum) pairs
-        const size_t rows = size_t(p.splits) * a->tokens * a->q_heads;
+        // weighted values, then their (maximum, sum) pairs
+        const size_t rows = size_t(p.splits) * size_t(plan.items - plan.whole) * plan.tile_rows;
         p.part_o = static_cast<float*>(a->workspace);
         p.part_ml = reinterpret_cast<float2*>(p.part_o + rows * a->cache->head_dim);
     }

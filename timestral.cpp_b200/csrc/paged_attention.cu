@@ -81,28 +81,6 @@ __device__ __forceinline__ void team_sync(int team) {
     else asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(32 * RG) : "memory");
 }
 
-// Division by a number known at launch: n / d for n < 2^31 as the high word of a product.
-struct FastDiv {
-    uint32_t d = 1, mul = 0, shift = 0;
-    FastDiv() = default;
-    explicit FastDiv(uint32_t divisor) : d(divisor) {
-        if (d == 1) return;
-        while ((1ull << shift) < d) ++shift;                       // mul = ceil(2^(31 + shift) / d) < 2^32
-        mul = uint32_t(((1ull << (31 + shift)) + d - 1) / d);
-        --shift;
-    }
-    __device__ __forceinline__ uint32_t div(uint32_t n) const { return d == 1 ? n : __umulhi(n, mul) >> shift; }
-    __device__ __forceinline__ uint32_t divmod(uint32_t n, uint32_t* rest) const {
-        const uint32_t x = div(n);
-        *rest = n - x * d;
-        return x;
-    }
-};
-struct RowsGrid {
-    FastDiv splits, heads, row_tiles, group;
-    uint32_t items = 0;
-};
-
 // What a team works on.
 struct RowTile {
     int seq, kvh, m0, rows;      // first row and live rows of the tile
@@ -140,21 +118,23 @@ __device__ __forceinline__ void quad_transpose(uint32_t (&v)[4]) {
 
 template <class T, int HD, int RG, int NR, bool JOIN>
 __global__ void __launch_bounds__(PR_THREADS)
-    paged_rows_kernel(const __grid_constant__ PageMaps maps, const PagedAttention a, const RowsGrid grid) {
+    paged_rows_kernel(const __grid_constant__ PageMaps maps, const PagedAttention a, const PagedGrid grid) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     using L = RowsLayout<HD, RG>;
     constexpr int KT = L::KT, MK = KT / 16, KS = HD / 16, MD = HD / 16, WR = 8 * NR, MT = WR * RG;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, rg = warp % RG, team = warp / RG;
 
-    // item = ((sequence, row tile), cached head, split)
-    const uint32_t item = blockIdx.x * (JOIN ? 1 : L::TEAMS) + (JOIN ? 0 : team);
-    if (item >= grid.items) return;
+    const uint32_t unit = blockIdx.x * (JOIN ? 1 : L::TEAMS) + (JOIN ? 0 : team);
+    if (unit >= grid.units) return;
     RowTile t;
-    uint32_t split, kvh, rt, seq = grid.row_tiles.divmod(grid.heads.divmod(grid.splits.divmod(item, &split), &kvh), &rt);
-    t.seq = int(seq);
-    t.kvh = int(kvh);
-    t.m0 = int(rt) * MT;
+    uint32_t split;
+    int splits;
+    const uint32_t item = unit_of(grid, unit, &split, &splits);
+    const PagedItem it = item_of(grid, item);
+    t.seq = it.seq;
+    t.kvh = it.kvh;
+    t.m0 = it.row_tile * MT;
     const SeqInfo q = load_seq(a.batch, t.seq, a.err);
     t.rows = min(MT, q.n * a.group - t.m0);
     if (t.rows <= 0) return;
@@ -165,7 +145,7 @@ __global__ void __launch_bounds__(PR_THREADS)
     t.lo = a.window ? max(0, t.base + t_first - a.window + 1) : 0;
     // this item's share of the tiles, and of those this team's
     const int tile0 = t.lo / KT, tiles = (t.hi + KT - 1) / KT - tile0;
-    const int share = int(grid.splits.div(tiles + a.splits - 1));
+    const int share = splits > 1 ? int(grid.splits.div(tiles + splits - 1)) : tiles;
     constexpr int STEP = JOIN ? L::TEAMS : 1;
     const int first = tile0 + int(split) * share + (JOIN ? team : 0), last = min(tile0 + (int(split) + 1) * share, tile0 + tiles);
 
@@ -379,7 +359,7 @@ __global__ void __launch_bounds__(PR_THREADS)
             sum[n][e] += __shfl_xor_sync(0xffffffffu, sum[n][e], 8);
             sum[n][e] += __shfl_xor_sync(0xffffffffu, sum[n][e], 16);
         }
-    const int64_t part = int64_t(split) * a.batch.tokens * a.q_heads;
+    const int64_t part = (int64_t(item - grid.whole) * splits + split) * MT;      // row 0 of the tile
     auto row_of = [&](int r, int64_t* token, int* head) {
         const int m = t.m0 + r, tok = int(grid.group.div(m));
         *token = t.start + tok;
@@ -388,14 +368,11 @@ __global__ void __launch_bounds__(PR_THREADS)
     if constexpr (!JOIN) {
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
-            if (a.splits > 1) {
+            if (splits > 1) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     if (pos[n][e] < 0) continue;
-                    int64_t token;
-                    int head;
-                    row_of(rg * WR + n * 8 + (lane & 3) * 2 + e, &token, &head);
-                    const int64_t at = part + token * a.q_heads + head;
+                    const int64_t at = part + rg * WR + n * 8 + (lane & 3) * 2 + e;
                     if (lane < 4) a.part_ml[at] = make_float2(mx[n][e], sum[n][e]);
                     if (mx[n][e] == -INFINITY) continue;
 #pragma unroll
@@ -471,11 +448,8 @@ __global__ void __launch_bounds__(PR_THREADS)
 #pragma unroll
             for (int e = 0; e < 8; ++e) y[e] = fmaf(src[e], f, y[e]);
         }
-        int64_t token;
-        int head;
-        row_of(r, &token, &head);
-        if (a.splits > 1) {
-            const int64_t at = part + token * a.q_heads + head;
+        if (splits > 1) {
+            const int64_t at = part + r;
             if (c == 0) a.part_ml[at] = make_float2(m, l);
             if (m != -INFINITY) {
                 float4* dst = reinterpret_cast<float4*>(a.part_o + at * HD + c * 8);
@@ -484,26 +458,33 @@ __global__ void __launch_bounds__(PR_THREADS)
             }
             continue;
         }
+        int64_t token;
+        int head;
+        row_of(r, &token, &head);
         store_row<T>(a, token, head, c, y, m == -INFINITY ? 0.f : 1.0f / l);
     }
 }
 
-// Join the splits of a (new token, query head) row: HD / 8 threads hold a partial row, G groups of
-// them share the splits out (8 for many splits of few rows, else 2), joined through shared memory.
+// Join the splits of a row: HD / 8 threads hold a partial row, G groups of them share the splits out
+// (8 for many splits of few rows, else 2), joined through shared memory.
 template <class T, int HD, int G>
-__global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttention a, const FastDiv chunk, const FastDiv heads) {
+__global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttention a, const PagedGrid grid, int tile_rows) {
     constexpr int CH = HD / 8, ROWS = 128 / (CH * G);
     __shared__ float so[ROWS * G][HD];
     __shared__ float2 sml[ROWS * G];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int slot = threadIdx.x / CH, c = threadIdx.x % CH, g = slot % G;
-    uint32_t i, head;
-    const uint32_t seq = chunk.divmod(heads.divmod(blockIdx.x * ROWS + slot / G, &head), &i);
-    SeqInfo q{};
-    if (seq < uint32_t(a.batch.seqs)) q = load_seq(a.batch, int(seq), nullptr);
-    const bool live = int(i) < q.n;
-    const int64_t token = q.start + i, at = token * a.q_heads + head, step = int64_t(a.batch.tokens) * a.q_heads;
-    float m = -INFINITY, y[8] = {}, l = 0.f;
+    // tile_rows is a power of two
+    const uint32_t row = blockIdx.x * ROWS + slot / G, split_item = row >> (31 - __clz(tile_rows)), r = row & (tile_rows - 1);
+    const PagedItem it = item_of(grid, min(grid.whole + split_item, grid.items - 1));
+    const SeqInfo q = load_seq(a.batch, it.seq, nullptr);
+    uint32_t in_group;
+    const int m = it.row_tile * tile_rows + int(r);
+    const int64_t token = q.start + int64_t(grid.group.divmod(m, &in_group));
+    const int head = it.kvh * a.group + int(in_group);
+    const bool live = grid.whole + split_item < grid.items && m < q.n * a.group;
+    const int64_t at = int64_t(split_item) * a.splits * tile_rows + r, step = tile_rows;
+    float top_m = -INFINITY, y[8] = {}, l = 0.f;
     if (live) {
 #pragma unroll 4
         for (int s = g; s < a.splits; s += G) {
@@ -511,8 +492,8 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttention
             if (ml.x == -INFINITY) continue;          // saw nothing: no partial row was written
             const float4* src = reinterpret_cast<const float4*>(a.part_o + (s * step + at) * HD + c * 8);
             const float4 u = src[0], w = src[1];
-            const float top = fmaxf(m, ml.x), f = exp2_ftz(ml.x - top), old = exp2_ftz(m - top);
-            m = top;
+            const float top = fmaxf(top_m, ml.x), f = exp2_ftz(ml.x - top), old = exp2_ftz(top_m - top);
+            top_m = top;
             l = fmaf(l, old, ml.y * f);
             const float p[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -521,7 +502,7 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttention
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) so[slot][c * 8 + e] = y[e];
-    if (c == 0) sml[slot] = make_float2(m, l);
+    if (c == 0) sml[slot] = make_float2(top_m, l);
     __syncthreads();
     if (g != 0 || !live) return;
     float top = -INFINITY;
@@ -539,7 +520,7 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttention
 #pragma unroll
         for (int e = 0; e < 8; ++e) y[e] = fmaf(so[slot + k][c * 8 + e], f, y[e]);
     }
-    store_row<T>(a, token, int(head), c, y, top == -INFINITY ? 0.f : 1.0f / l);
+    store_row<T>(a, token, head, c, y, top == -INFINITY ? 0.f : 1.0f / l);
 }
 
 // Rows of a problem -> warps of a team and their rows: 8, 16, 32 or 64 rows.
@@ -549,7 +530,7 @@ int rows_of_team(const PagedAttention& a) {
 }
 
 template <class T, int HD, int RG, int NR, bool JOIN>
-cudaError_t launch_rows(const PagedAttention& a, cudaStream_t stream) {
+cudaError_t launch_rows(const PagedAttention& a, const PagedGrid& grid, cudaStream_t stream) {
     using L = RowsLayout<HD, RG>;
     static KernelSetup configured;
     int dev = 0;
@@ -560,36 +541,27 @@ cudaError_t launch_rows(const PagedAttention& a, cudaStream_t stream) {
         if (e != cudaSuccess) return e;
         configured.done(dev, key);
     }
-    constexpr int MT = 8 * NR * RG;
-    const int64_t row_tiles = (int64_t(a.batch.max_chunk) * a.group + MT - 1) / MT;
-    const int64_t items = row_tiles * a.cache.kv_heads * a.batch.seqs * a.splits;
-    if (items > INT32_MAX - 4) return cudaErrorInvalidValue;
     PageMaps maps;
     if (!page_maps(&maps, a.cache, std::is_same<T, __nv_bfloat16>::value, L::KT)) return cudaErrorInvalidValue;
-    RowsGrid grid;
-    grid.splits = FastDiv(a.splits);
-    grid.heads = FastDiv(a.cache.kv_heads);
-    grid.row_tiles = FastDiv(uint32_t(row_tiles));
-    grid.group = FastDiv(a.group);
-    grid.items = uint32_t(items);
-    const unsigned blocks = unsigned(JOIN ? items : (items + L::TEAMS - 1) / L::TEAMS);
+    const unsigned blocks = JOIN ? grid.units : (grid.units + L::TEAMS - 1) / L::TEAMS;
     paged_rows_kernel<T, HD, RG, NR, JOIN><<<blocks, PR_THREADS, L::SMEM, stream>>>(maps, a, grid);
     return cudaGetLastError();
 }
 template <class T, int HD>
-cudaError_t dispatch_rows(const PagedAttention& a, bool join, cudaStream_t stream) {
-    switch (rows_of_team(a)) {
-        case 8: return join ? launch_rows<T, HD, 1, 1, true>(a, stream) : launch_rows<T, HD, 1, 1, false>(a, stream);
-        case 16: return join ? launch_rows<T, HD, 1, 2, true>(a, stream) : launch_rows<T, HD, 1, 2, false>(a, stream);
-        case 32: return join ? launch_rows<T, HD, 2, 2, true>(a, stream) : launch_rows<T, HD, 2, 2, false>(a, stream);
-        default: return launch_rows<T, HD, 4, 2, false>(a, stream);     // one team
+cudaError_t dispatch_rows(const PagedAttention& a, const PagedGrid& grid, const PagedPlan& plan, cudaStream_t stream) {
+    const bool join = plan.join;
+    switch (plan.tile_rows) {
+        case 8: return join ? launch_rows<T, HD, 1, 1, true>(a, grid, stream) : launch_rows<T, HD, 1, 1, false>(a, grid, stream);
+        case 16: return join ? launch_rows<T, HD, 1, 2, true>(a, grid, stream) : launch_rows<T, HD, 1, 2, false>(a, grid, stream);
+        case 32: return join ? launch_rows<T, HD, 2, 2, true>(a, grid, stream) : launch_rows<T, HD, 2, 2, false>(a, grid, stream);
+        default: return launch_rows<T, HD, 4, 2, false>(a, grid, stream);     // one team
     }
 }
 
 template <class T, int HD, int G>
-cudaError_t launch_combine(const PagedAttention& a, cudaStream_t stream) {
+cudaError_t launch_combine(const PagedAttention& a, const PagedGrid& grid, int tile_rows, cudaStream_t stream) {
     constexpr int ROWS = 128 / (HD / 8 * G);
-    const int64_t rows = int64_t(a.batch.max_chunk) * a.q_heads * a.batch.seqs;
+    const int64_t rows = int64_t(grid.items - grid.whole) * tile_rows;
     if (rows > INT32_MAX - ROWS) return cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned((rows + ROWS - 1) / ROWS));
@@ -600,16 +572,15 @@ cudaError_t launch_combine(const PagedAttention& a, cudaStream_t stream) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, paged_combine_kernel<T, HD, G>, a, FastDiv(a.batch.max_chunk), FastDiv(a.q_heads));
+    return cudaLaunchKernelEx(&cfg, paged_combine_kernel<T, HD, G>, a, grid, tile_rows);
 }
 
 template <class T, int HD>
-cudaError_t dispatch(const PagedAttention& a, cudaStream_t stream) {
-    const PagedPlan plan = paged_plan(a);
-    const cudaError_t e = plan.tiles ? paged_attention_tiles(a, std::is_same<T, __nv_bfloat16>::value, stream)
-                                     : dispatch_rows<T, HD>(a, plan.join, stream);
+cudaError_t dispatch(const PagedAttention& a, const PagedPlan& plan, const PagedGrid& grid, cudaStream_t stream) {
+    const cudaError_t e = plan.tiles ? paged_attention_tiles(a, grid, std::is_same<T, __nv_bfloat16>::value, stream)
+                                     : dispatch_rows<T, HD>(a, grid, plan, stream);
     if (e != cudaSuccess || a.splits == 1) return e;
-    return a.splits > 4 ? launch_combine<T, HD, 8>(a, stream) : launch_combine<T, HD, 2>(a, stream);
+    return a.splits > 4 ? launch_combine<T, HD, 8>(a, grid, plan.tile_rows, stream) : launch_combine<T, HD, 2>(a, grid, plan.tile_rows, stream);
 }
 
 }  // namespace
@@ -638,25 +609,47 @@ bool page_maps(PageMaps* m, const PagedCache& c, bool bf16, int box_slots) {
 
 PagedPlan paged_plan(const PagedAttention& a) {
     PagedPlan p;
-    p.tiles = int64_t(a.batch.max_chunk) * a.group > 64;
     const int64_t rows = int64_t(a.batch.max_chunk) * a.group;
-    const int mt = p.tiles ? kPagedTileRows : rows_of_team(a);
-    const int64_t items = (rows + mt - 1) / mt * a.cache.kv_heads * a.batch.seqs;
-    const int keys = a.window ? int(std::min<int64_t>(a.batch.max_length, int64_t(a.window) + a.batch.max_chunk)) : a.batch.max_length;
+    p.tiles = rows > 64;
+    p.tile_rows = p.tiles ? kPagedTileRows : rows_of_team(a);
+    p.row_tiles = (rows + p.tile_rows - 1) / p.tile_rows;
+    p.items = p.row_tiles * a.cache.kv_heads * a.batch.seqs;
     const int64_t sms = device_sm_count();
+    const int64_t keys = a.window ? std::min<int64_t>(a.batch.max_length, int64_t(a.window) + a.batch.max_chunk) : a.batch.max_length;
     if (p.tiles) {
-        p.splits = int(std::max<int64_t>(1, std::min<int64_t>({(sms + items - 1) / items, (keys + 511) / 512, 256})));
+        // As many items as fill the SMs once or more stay whole; the rest are split so that they take the
+        // least time together: rounds of blocks times a block's key tiles, of which its start and end cost
+        // about three more (and the join about four).
+        p.whole = p.items / sms * sms;
+        const int64_t rest = p.items - p.whole, tiles = (keys + 127) / 128;
+        int64_t best = INT64_MAX;
+        for (int s = 1; rest && s <= 32 && (s == 1 || 2 * s <= tiles); ++s) {
+            const int64_t cost = (rest * s + sms - 1) / sms * ((tiles + s - 1) / s + 3) + (s > 1 ? 4 : 0);
+            if (cost < best) { best = cost; p.splits = s; }
+        }
     } else {
         p.join = rows <= 32 && keys > 256;
-        p.splits = int(std::max<int64_t>(1, std::min<int64_t>({items >= sms ? (4 * sms + items - 1) / items : sms / items, (keys + 255) / 256, 256})));
+        p.splits = int(std::max<int64_t>(1, std::min<int64_t>({p.items >= sms ? (4 * sms + p.items - 1) / p.items : sms / p.items, (keys + 255) / 256, 256})));
     }
-    p.split_bytes = size_t(a.batch.tokens) * a.q_heads * (size_t(a.cache.head_dim) * 4 + 8);
+    p.split_bytes = size_t(p.items - p.whole) * p.tile_rows * (size_t(a.cache.head_dim) * 4 + 8);
     return p;
 }
 
 cudaError_t paged_attention(const PagedAttention& a, bool bf16, cudaStream_t stream) {
-    if (a.cache.head_dim == 64) return bf16 ? dispatch<__nv_bfloat16, 64>(a, stream) : dispatch<__half, 64>(a, stream);
-    return bf16 ? dispatch<__nv_bfloat16, 128>(a, stream) : dispatch<__half, 128>(a, stream);
+    const PagedPlan p = paged_plan(a);
+    const int64_t whole = a.splits > 1 ? p.whole : p.items, units = whole + (p.items - whole) * a.splits;
+    if (units > INT32_MAX - 4) return cudaErrorInvalidValue;
+    PagedGrid g;
+    g.splits = FastDiv(uint32_t(a.splits));
+    g.heads = FastDiv(uint32_t(a.cache.kv_heads));
+    g.seqs = FastDiv(uint32_t(a.batch.seqs));
+    g.group = FastDiv(uint32_t(a.group));
+    g.items = uint32_t(p.items);
+    g.whole = uint32_t(whole);
+    g.units = uint32_t(units);
+    g.row_tiles = uint32_t(p.row_tiles);
+    if (a.cache.head_dim == 64) return bf16 ? dispatch<__nv_bfloat16, 64>(a, p, g, stream) : dispatch<__half, 64>(a, p, g, stream);
+    return bf16 ? dispatch<__nv_bfloat16, 128>(a, p, g, stream) : dispatch<__half, 128>(a, p, g, stream);
 }
 
 }  // namespace tsb

@@ -132,7 +132,7 @@ __device__ __forceinline__ void exp2_poly(F2 x, float& r0, float& r1) {
 
 template <class T, int HD>
 __global__ void __launch_bounds__(PT_THREADS, 1)
-    paged_tiles_kernel(const __grid_constant__ PageMaps maps, const PagedAttention a, int row_tiles) {
+    paged_tiles_kernel(const __grid_constant__ PageMaps maps, const PagedAttention a, const PagedGrid grid) {
     using L = TilesLayout<HD>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* qbuf = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -141,23 +141,21 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     volatile int* abort = &bars->abort;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
-    // the block's rows; the row tiles that see most keys come first
-    const int split = int(blockIdx.x % a.splits);
-    int b = int(blockIdx.x / a.splits);
-    const int per = a.cache.kv_heads * a.batch.seqs;
-    const int m0 = (row_tiles - 1 - b / per) * kPagedTileRows;
-    b %= per;
-    const int kvh = b % a.cache.kv_heads, seq = b / a.cache.kv_heads;
+    uint32_t split;
+    int splits;
+    const uint32_t item = unit_of(grid, blockIdx.x, &split, &splits);
+    const PagedItem it = item_of(grid, item);
+    const int m0 = it.row_tile * kPagedTileRows, kvh = it.kvh, seq = it.seq;
     const SeqInfo q = load_seq(a.batch, seq, a.err);
     const int rows = min(kPagedTileRows, q.n * a.group - m0);
     if (rows <= 0) return;
     const int base = q.len - q.n;
-    auto position = [&](int r) { return base + (m0 + r) / a.group; };
+    auto position = [&](int r) { return base + int(grid.group.div(m0 + r)); };
     const int hi = position(rows - 1) + 1;
     const int lo = a.window ? max(0, position(0) - a.window + 1) : 0;
     const int tile0 = lo / PT_KT, tiles = (hi + PT_KT - 1) / PT_KT - tile0;
-    const int share = (tiles + a.splits - 1) / a.splits;
-    const int first = tile0 + split * share, n = min(share, tile0 + tiles - first);
+    const int share = splits > 1 ? int(grid.splits.div(tiles + splits - 1)) : tiles;
+    const int first = tile0 + int(split) * share, n = min(share, tile0 + tiles - first);
     // key tiles of each row tile in this block's share
     int ng[2];
 #pragma unroll
@@ -170,9 +168,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     const int t = threadIdx.x & 127, g = threadIdx.x >> 7;         // (warps 0-7)
     const int row = g * 128 + t;
     const bool live = warp < 8 && row < rows;
-    const int64_t token = q.start + (m0 + row) / a.group;
-    const int head = kvh * a.group + (m0 + row) % a.group;
-    const int64_t part = (int64_t(split) * a.batch.tokens + token) * a.q_heads + head;
+    uint32_t in_group;
+    const int64_t token = q.start + int64_t(grid.group.divmod(m0 + row, &in_group));
+    const int head = kvh * a.group + int(in_group);
+    const int64_t part = (int64_t(item - grid.whole) * splits + split) * kPagedTileRows + row;
     if (nt == 0) {                                                  // (only with splits)
         if (live) a.part_ml[part] = make_float2(-INFINITY, 0.f);
         return;
@@ -411,8 +410,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
         if (ok) {
             tc_fence_after();
             const bool none = ngg == 0;
-            if (a.splits > 1 && live) a.part_ml[part] = none ? make_float2(-INFINITY, 0.f) : make_float2(mref, sum);
-            const float inv = none || mref == -INFINITY ? 0.f : a.splits > 1 ? 1.f : 1.0f / sum;
+            if (splits > 1 && live) a.part_ml[part] = none ? make_float2(-INFINITY, 0.f) : make_float2(mref, sum);
+            const float inv = none || mref == -INFINITY ? 0.f : splits > 1 ? 1.f : 1.0f / sum;
             const T* gate = a.gate.data ? static_cast<const T*>(a.gate.data) + token * a.gate.token + head * a.gate.head : nullptr;
             T* out = static_cast<T*>(a.out.data) + token * a.out.token + head * a.out.head;
 #pragma unroll 1
@@ -426,7 +425,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                     tmem_ld_wait();
                 }
                 if (!live) continue;
-                if (a.splits > 1) {
+                if (splits > 1) {
                     if (none) continue;
                     float4* dst = reinterpret_cast<float4*>(a.part_o + part * HD + c0);
 #pragma unroll
@@ -458,7 +457,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
 }
 
 template <class T, int HD>
-cudaError_t launch_tiles(const PagedAttention& a, cudaStream_t stream) {
+cudaError_t launch_tiles(const PagedAttention& a, const PagedGrid& grid, cudaStream_t stream) {
     using L = TilesLayout<HD>;
     const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
     const PagedCache& c = a.cache;
@@ -478,19 +477,16 @@ cudaError_t launch_tiles(const PagedAttention& a, cudaStream_t stream) {
         if (fa.numRegs < PT_LAUNCH_REGS) return cudaErrorLaunchOutOfResources;
         configured.done(dev, key);
     }
-    const int64_t row_tiles = (int64_t(a.batch.max_chunk) * a.group + kPagedTileRows - 1) / kPagedTileRows;
-    const int64_t blocks = row_tiles * c.kv_heads * a.batch.seqs * a.splits;
-    if (blocks > INT32_MAX) return cudaErrorInvalidValue;
-    paged_tiles_kernel<T, HD><<<unsigned(blocks), PT_THREADS, L::SMEM, stream>>>(maps, a, int(row_tiles));
+    paged_tiles_kernel<T, HD><<<grid.units, PT_THREADS, L::SMEM, stream>>>(maps, a, grid);
     return cudaGetLastError();
 }
 
 }  // namespace
 
-cudaError_t paged_attention_tiles(const PagedAttention& a, bool bf16, cudaStream_t stream) {
+cudaError_t paged_attention_tiles(const PagedAttention& a, const PagedGrid& grid, bool bf16, cudaStream_t stream) {
     if (a.cache.head_dim == 64)
-        return bf16 ? launch_tiles<__nv_bfloat16, 64>(a, stream) : launch_tiles<__half, 64>(a, stream);
-    return bf16 ? launch_tiles<__nv_bfloat16, 128>(a, stream) : launch_tiles<__half, 128>(a, stream);
+        return bf16 ? launch_tiles<__nv_bfloat16, 64>(a, grid, stream) : launch_tiles<__half, 64>(a, grid, stream);
+    return bf16 ? launch_tiles<__nv_bfloat16, 128>(a, grid, stream) : launch_tiles<__half, 128>(a, grid, stream);
 }
 
 }  // namespace tsb

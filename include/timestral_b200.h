@@ -173,8 +173,8 @@ TIMESTRAL_API int tsb_refine_static(const float* d_q, const float* d_rows, const
  * TSB_ERR_ARG), as is `stream` (cudaStream_t, NULL = legacy default stream). Calls enqueue
  * work and return; they allocate nothing, keep nothing between calls and may be captured into
  * a CUDA graph. Values are f16 or bf16, sums and statistics f32, each result is rounded once.
- * The last axis (head_dim) is contiguous; every data pointer is 16-byte aligned and every
- * stride, in elements, a multiple of 8. Offsets are 64-bit. Argument errors go to
+ * The last axis (head_dim) is contiguous; every pointer to values, weights or angles is 16-byte
+ * aligned and every stride of values, in elements, a multiple of 8. Offsets are 64-bit. Argument errors go to
  * timestral_capi_last_error(NULL).
  *
  * What only the device can see (positions, page numbers, lengths) is checked there: `error`

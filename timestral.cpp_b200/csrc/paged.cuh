@@ -10,6 +10,24 @@
 
 namespace tsb {
 
+// Division by a number known at launch: n / d for n < 2^31 as the high word of a product.
+struct FastDiv {
+    uint32_t d = 1, mul = 0, shift = 0;
+    FastDiv() = default;
+    explicit FastDiv(uint32_t divisor) : d(divisor) {
+        if (d == 1) return;
+        while ((1ull << shift) < d) ++shift;                       // mul = ceil(2^(31 + shift) / d) < 2^32
+        mul = uint32_t(((1ull << (31 + shift)) + d - 1) / d);
+        --shift;
+    }
+    __device__ __forceinline__ uint32_t div(uint32_t n) const { return d == 1 ? n : __umulhi(n, mul) >> shift; }
+    __device__ __forceinline__ uint32_t divmod(uint32_t n, uint32_t* rest) const {
+        const uint32_t x = div(n);
+        *rest = n - x * d;
+        return x;
+    }
+};
+
 // [tokens][heads][head_dim], strides in elements.
 struct PagedHeads {
     void* data = nullptr;
@@ -43,6 +61,7 @@ struct NormRopeSide {
     PagedHeads in, out;
     const float* weight = nullptr;
     int heads = 0;
+    FastDiv units;                      // threads' worth of heads of a token (set by the launch)
 };
 struct NormRope {
     NormRopeSide q, k;
@@ -75,24 +94,6 @@ struct PagedAttention {
     float* part_o = nullptr;            // [items - whole][splits][tile_rows][head_dim], unnormalised
     float2* part_ml = nullptr;          // the same rows: reference maximum (log2 units), sum
     int* err = nullptr;
-};
-
-// Division by a number known at launch: n / d for n < 2^31 as the high word of a product.
-struct FastDiv {
-    uint32_t d = 1, mul = 0, shift = 0;
-    FastDiv() = default;
-    explicit FastDiv(uint32_t divisor) : d(divisor) {
-        if (d == 1) return;
-        while ((1ull << shift) < d) ++shift;                       // mul = ceil(2^(31 + shift) / d) < 2^32
-        mul = uint32_t(((1ull << (31 + shift)) + d - 1) / d);
-        --shift;
-    }
-    __device__ __forceinline__ uint32_t div(uint32_t n) const { return d == 1 ? n : __umulhi(n, mul) >> shift; }
-    __device__ __forceinline__ uint32_t divmod(uint32_t n, uint32_t* rest) const {
-        const uint32_t x = div(n);
-        *rest = n - x * d;
-        return x;
-    }
 };
 
 // The work of a call: an item is a tile of rows of one (sequence, cached head), those with the last

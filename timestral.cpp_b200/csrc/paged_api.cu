@@ -213,7 +213,7 @@ extern "C" TIMESTRAL_API int tsb_norm_rope(const tsb_norm_rope_args* a, void* st
         {a->q, a->q_out, a->q_weight, a->q_heads, "q", "q_out", "q_weight"}, {a->k, a->k_out, a->k_weight, a->k_heads, "k", "k_out", "k_weight"}};
     for (const auto& s : side)
         if (s.heads && (!heads_shape(r, s.in, s.name, s.heads, a->head_dim) || !output_shape(r, s.out, s.out_name, a->tokens, s.heads, a->head_dim) ||
-                        !aligned(r, s.w, s.w_name, 4)))
+                        !aligned(r, s.w, s.w_name, 16)))
             return r.report();
     if (!a->tokens || (!a->q_heads && !a->k_heads)) return TSB_OK;
     int dev = 0;
@@ -238,7 +238,7 @@ extern "C" TIMESTRAL_API int tsb_paged_append(const tsb_paged_append_args* a, vo
     Refusal r("tsb_paged_append");
     if (!r.need(a != nullptr, "args is NULL") || !cache_shape(r, a->cache) || !batch_shape(r, a->batch, a->cache, a->tokens) ||
         !heads_shape(r, a->k, "k", a->cache->kv_heads, a->cache->head_dim) || !heads_shape(r, a->v, "v", a->cache->kv_heads, a->cache->head_dim) ||
-        !aligned(r, a->k_weight, "k_weight", 4) || !r.need(std::isfinite(a->eps) && a->eps >= 0, "eps is negative or not finite") ||
+        !aligned(r, a->k_weight, "k_weight", 16) || !r.need(std::isfinite(a->eps) && a->eps >= 0, "eps is negative or not finite") ||
         !rotation_shape(r, a->rotation, a->cache->head_dim, false))
         return r.report();
     if (!a->tokens || !a->batch->seqs || !a->batch->max_chunk) return TSB_OK;

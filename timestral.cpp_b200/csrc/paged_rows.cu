@@ -8,6 +8,9 @@
 // a shuffle over PT lanes.
 #include "paged.cuh"
 
+#include <algorithm>
+#include <climits>
+
 namespace tsb {
 namespace {
 
@@ -22,23 +25,18 @@ __device__ __forceinline__ void pair_at(int p, int rope_dim, int* a, int* b) {
 // Every thread of the head's PT lanes takes part (live: it holds values).
 template <int PT>
 __device__ __forceinline__ void norm_turn(float (&x)[8], float (&y)[8], bool normed, const float (&w0)[8], const float (&w1)[8],
-                                          float eps, int head_dim, bool turned, const float* c, const float* s) {
+                                          float eps, float inv_dim, bool turned, const float (&cc)[8], const float (&sn)[8]) {
     if (normed) {
         float ss = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], fmaf(y[i], y[i], ss));
 #pragma unroll
         for (int o = PT / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o, PT);
-        const float r = 1.0f / sqrtf(ss / float(head_dim) + eps);
+        const float r = rsqrtf(fmaf(ss, inv_dim, eps));
 #pragma unroll
         for (int i = 0; i < 8; ++i) { x[i] = x[i] * r * w0[i]; y[i] = y[i] * r * w1[i]; }
     }
     if (turned) {
-        float cc[8], sn[8];
-        *reinterpret_cast<float4*>(cc) = *reinterpret_cast<const float4*>(c);
-        *reinterpret_cast<float4*>(cc + 4) = *reinterpret_cast<const float4*>(c + 4);
-        *reinterpret_cast<float4*>(sn) = *reinterpret_cast<const float4*>(s);
-        *reinterpret_cast<float4*>(sn + 4) = *reinterpret_cast<const float4*>(s + 4);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float a = x[i], b = y[i];
@@ -48,126 +46,160 @@ __device__ __forceinline__ void norm_turn(float (&x)[8], float (&y)[8], bool nor
     }
 }
 
-__device__ __forceinline__ void load_weight(const float* w, int a, int b, float (&w0)[8], float (&w1)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) { w0[i] = w[a + i]; w1[i] = w[b + i]; }
+__device__ __forceinline__ void load8(const float* p, float (&f)[8]) {
+    *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(p);
+    *reinterpret_cast<float4*>(f + 4) = *reinterpret_cast<const float4*>(p + 4);
 }
 
 constexpr int kThreads = 256;
 
-// blocks [0, q_blocks) norm and turn the queries, the rest the keys. Item = (token, head).
+// Blocks [0, q_blocks) norm and turn the queries, the rest the keys. A thread has U heads of one
+// token, which share its angles and weights: their table rows (f32, twice the bytes of a 16-bit head)
+// come from L1 once for U heads, and 32 U bytes of values are in flight per thread.
 template <class T, int PT, int U>
-__global__ void __launch_bounds__(kThreads) norm_rope_kernel(const NormRope a, int q_blocks) {
+__global__ void __launch_bounds__(kThreads, U == 1 ? 4 : 3) norm_rope_kernel(const NormRope a, int q_blocks, float inv_dim) {
     const bool is_q = int(blockIdx.x) < q_blocks;
     const NormRopeSide& s = is_q ? a.q : a.k;
-    const int64_t block = is_q ? blockIdx.x : int(blockIdx.x) - q_blocks;
-    constexpr int HEADS = kThreads / PT;
+    const uint32_t block = is_q ? blockIdx.x : blockIdx.x - q_blocks;
     const int p = threadIdx.x % PT;
-    const int64_t first = block * (HEADS * U) + threadIdx.x / PT, items = int64_t(a.tokens) * s.heads;
-    const bool holds = p < a.head_dim / 16;
+    const uint32_t unit = block * (kThreads / PT) + threadIdx.x / PT;
+    uint32_t first;
+    const uint32_t token = s.units.divmod(unit, &first);
+    first *= U;
+    const bool here = token < uint32_t(a.tokens) && p < a.head_dim / 16;
     int e0, e1;
-    pair_at(holds ? p : 0, a.rot.dim, &e0, &e1);
+    pair_at(p < a.head_dim / 16 ? p : 0, a.rot.dim, &e0, &e1);
     uint4 u0[U], u1[U];
-    int64_t to[U];
-    int row[U];
-    bool live[U];
+    const T* in = static_cast<const T*>(s.in.data) + int64_t(token) * s.in.token + first * s.in.head;
 #pragma unroll
     for (int j = 0; j < U; ++j) {
-        const int64_t item = first + j * HEADS;
-        live[j] = item < items && holds;
-        row[j] = -1;
         u0[j] = u1[j] = make_uint4(0, 0, 0, 0);
-        to[j] = 0;
-        if (!live[j]) continue;
-        const int64_t token = item / s.heads;
-        const int head = int(item - token * s.heads);
-        const T* in = static_cast<const T*>(s.in.data) + token * s.in.token + head * s.in.head;
-        u0[j] = *reinterpret_cast<const uint4*>(in + e0);
-        u1[j] = *reinterpret_cast<const uint4*>(in + e1);
-        to[j] = token * s.out.token + head * s.out.head;
-        if (a.rot.cos) {
-            row[j] = a.rot.positions[token];
-            if (row[j] < 0 || row[j] >= a.rot.rows) { record_error(a.err, kDevBadShape); live[j] = false; row[j] = -1; }
+        if (!here || int(first) + j >= s.heads) continue;
+        u0[j] = *reinterpret_cast<const uint4*>(in + j * s.in.head + e0);
+        u1[j] = *reinterpret_cast<const uint4*>(in + j * s.in.head + e1);
+    }
+    bool writes = here, turned = false;
+    float c[8] = {}, sn[8] = {}, w0[8] = {}, w1[8] = {};
+    if (here && a.rot.cos) {
+        const int row = a.rot.positions[token];
+        if (row < 0 || row >= a.rot.rows) { record_error(a.err, kDevBadShape); writes = false; }
+        turned = writes && e0 < a.rot.dim;
+        if (turned) {
+            load8(a.rot.cos + row * a.rot.stride + e0, c);
+            load8(a.rot.sin + row * a.rot.stride + e0, sn);
         }
     }
-    float w0[8] = {}, w1[8] = {};
-    if (s.weight && holds) load_weight(s.weight, e0, e1, w0, w1);
+    if (s.weight) {
+        load8(s.weight + e0, w0);
+        load8(s.weight + e1, w1);
+    }
+    T* out = static_cast<T*>(s.out.data) + int64_t(token) * s.out.token + first * s.out.head;
 #pragma unroll
     for (int j = 0; j < U; ++j) {
         float x[8], y[8];
         unpack8<T>(u0[j], x);
         unpack8<T>(u1[j], y);
-        const int64_t at = int64_t(row[j]) * a.rot.stride + e0;
-        norm_turn<PT>(x, y, s.weight != nullptr, w0, w1, a.eps, a.head_dim, row[j] >= 0 && e0 < a.rot.dim, a.rot.cos + at,
-                      a.rot.sin + at);
-        if (!live[j]) continue;
-        T* out = static_cast<T*>(s.out.data) + to[j];
-        *reinterpret_cast<uint4*>(out + e0) = pack8<T>(x);
-        *reinterpret_cast<uint4*>(out + e1) = pack8<T>(y);
+        norm_turn<PT>(x, y, s.weight != nullptr, w0, w1, a.eps, inv_dim, turned, c, sn);
+        if (!writes || int(first) + j >= s.heads) continue;
+        *reinterpret_cast<uint4*>(out + j * s.out.head + e0) = pack8<T>(x);
+        *reinterpret_cast<uint4*>(out + j * s.out.head + e1) = pack8<T>(y);
     }
 }
 
-// One block: the next kThreads / PT (token, head) items of a sequence, its keys and its values.
-template <class T, int PT>
-__global__ void __launch_bounds__(kThreads) paged_append_kernel(const PagedAppend a, int blocks_per_seq) {
-    const int seq = blockIdx.x / blocks_per_seq;
+// A block: new tokens of one sequence, U cached heads a thread, their keys and values.
+template <class T, int PT, int U>
+__global__ void __launch_bounds__(kThreads, U == 1 ? 4 : 3)
+    paged_append_kernel(const PagedAppend a, const FastDiv blocks, const FastDiv units, float inv_dim) {
+    uint32_t in_seq, first;
+    const int seq = int(blocks.divmod(blockIdx.x, &in_seq));
     const SeqInfo q = load_seq(a.batch, seq, a.err);
     const PagedCache& c = a.cache;
-    constexpr int HEADS = kThreads / PT;
-    const int64_t item = int64_t(blockIdx.x % blocks_per_seq) * HEADS + threadIdx.x / PT;
     const int p = threadIdx.x % PT;
-    const int i = int(item / c.kv_heads), head = int(item - int64_t(i) * c.kv_heads);
+    const int i = int(units.divmod(in_seq * (kThreads / PT) + threadIdx.x / PT, &first));
+    first *= U;
     const bool live = i < q.n;
     if (!__any_sync(0xffffffffu, live)) return;
     int e0, e1;
     pair_at(p, a.rot.dim, &e0, &e1);
-    uint4 k0 = make_uint4(0, 0, 0, 0), k1 = k0, v0 = k0, v1 = k0;
-    int page = -1, pos = 0, row = -1;
-    bool writes = live;
-    if (live) {
-        const int64_t token = q.start + i;
-        const T* k = static_cast<const T*>(a.k.data) + token * a.k.token + head * a.k.head;
-        const T* v = static_cast<const T*>(a.v.data) + token * a.v.token + head * a.v.head;
-        pos = q.len - q.n + i;
-        page = c.table[int64_t(seq) * c.table_stride + (pos >> c.page_shift)];
-        k0 = *reinterpret_cast<const uint4*>(k + e0);
-        k1 = *reinterpret_cast<const uint4*>(k + e1);
-        v0 = *reinterpret_cast<const uint4*>(v + e0);
-        v1 = *reinterpret_cast<const uint4*>(v + e1);
-        if (page < 0 || page >= c.num_pages) { record_error(a.err, kDevBadPage); writes = false; }
-        if (a.rot.cos) {
-            row = a.rot.positions ? a.rot.positions[token] : pos;
-            if (row < 0 || row >= a.rot.rows) { record_error(a.err, kDevBadShape); writes = false; row = -1; }
-        }
+    const int64_t token = q.start + i;
+    const int pos = q.len - q.n + i;
+    uint4 k0[U], k1[U], v0[U], v1[U];
+    int page = -1;
+    if (live) page = c.table[int64_t(seq) * c.table_stride + (pos >> c.page_shift)];
+    const T* k = static_cast<const T*>(a.k.data) + token * a.k.token + first * a.k.head;
+    const T* v = static_cast<const T*>(a.v.data) + token * a.v.token + first * a.v.head;
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+        k0[j] = k1[j] = v0[j] = v1[j] = make_uint4(0, 0, 0, 0);
+        if (!live || int(first) + j >= c.kv_heads) continue;
+        k0[j] = *reinterpret_cast<const uint4*>(k + j * a.k.head + e0);
+        k1[j] = *reinterpret_cast<const uint4*>(k + j * a.k.head + e1);
+        v0[j] = *reinterpret_cast<const uint4*>(v + j * a.v.head + e0);
+        v1[j] = *reinterpret_cast<const uint4*>(v + j * a.v.head + e1);
     }
+    bool writes = live;
+    if (live && (page < 0 || page >= c.num_pages)) { record_error(a.err, kDevBadPage); writes = false; }
     if (a.k_weight || a.rot.cos) {
-        float x[8], y[8], w0[8] = {}, w1[8] = {};
-        unpack8<T>(k0, x);
-        unpack8<T>(k1, y);
-        if (a.k_weight) load_weight(a.k_weight, e0, e1, w0, w1);
-        const int64_t at = int64_t(row) * a.rot.stride + e0;
-        norm_turn<PT>(x, y, a.k_weight != nullptr, w0, w1, a.eps, c.head_dim, row >= 0 && e0 < a.rot.dim, a.rot.cos + at,
-                      a.rot.sin + at);
-        k0 = pack8<T>(x);
-        k1 = pack8<T>(y);
+        float cs[8] = {}, sn[8] = {}, w0[8] = {}, w1[8] = {};
+        bool turned = false;
+        if (live && a.rot.cos) {
+            const int row = a.rot.positions ? a.rot.positions[token] : pos;
+            if (row < 0 || row >= a.rot.rows) { record_error(a.err, kDevBadShape); writes = false; }
+            turned = writes && e0 < a.rot.dim;
+            if (turned) {
+                load8(a.rot.cos + row * a.rot.stride + e0, cs);
+                load8(a.rot.sin + row * a.rot.stride + e0, sn);
+            }
+        }
+        if (a.k_weight) {
+            load8(a.k_weight + e0, w0);
+            load8(a.k_weight + e1, w1);
+        }
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            float x[8], y[8];
+            unpack8<T>(k0[j], x);
+            unpack8<T>(k1[j], y);
+            norm_turn<PT>(x, y, a.k_weight != nullptr, w0, w1, a.eps, inv_dim, turned, cs, sn);
+            k0[j] = pack8<T>(x);
+            k1[j] = pack8<T>(y);
+        }
     }
     if (!writes) return;
     const int slot = pos & ((1 << c.page_shift) - 1);
-    T* kd = static_cast<T*>(c.k) + page * c.k_page + head * c.k_head + slot * c.k_slot;
-    T* vd = static_cast<T*>(c.v) + page * c.v_page + head * c.v_head + slot * c.v_slot;
-    *reinterpret_cast<uint4*>(kd + e0) = k0;
-    *reinterpret_cast<uint4*>(kd + e1) = k1;
-    *reinterpret_cast<uint4*>(vd + e0) = v0;
-    *reinterpret_cast<uint4*>(vd + e1) = v1;
+    T* kd = static_cast<T*>(c.k) + page * c.k_page + first * c.k_head + slot * c.k_slot;
+    T* vd = static_cast<T*>(c.v) + page * c.v_page + first * c.v_head + slot * c.v_slot;
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+        if (int(first) + j >= c.kv_heads) break;
+        *reinterpret_cast<uint4*>(kd + j * c.k_head + e0) = k0[j];
+        *reinterpret_cast<uint4*>(kd + j * c.k_head + e1) = k1[j];
+        *reinterpret_cast<uint4*>(vd + j * c.v_head + e0) = v0[j];
+        *reinterpret_cast<uint4*>(vd + j * c.v_head + e1) = v1[j];
+    }
 }
 
+template <class T, int PT, int U>
+cudaError_t launch_norm_rope(const NormRope& a, cudaStream_t stream) {
+    constexpr int PER = kThreads / PT;
+    NormRope n = a;
+    int64_t blocks[2];
+    NormRopeSide* side[2] = {&n.q, &n.k};
+    for (int i = 0; i < 2; ++i) {
+        const int64_t units = (side[i]->heads + U - 1) / U;
+        side[i]->units = FastDiv(uint32_t(units > 0 ? units : 1));
+        blocks[i] = (units * a.tokens + PER - 1) / PER;
+    }
+    if ((blocks[0] + blocks[1]) * PER > INT32_MAX) return cudaErrorInvalidValue;
+    norm_rope_kernel<T, PT, U><<<unsigned(blocks[0] + blocks[1]), kThreads, 0, stream>>>(n, int(blocks[0]), 1.0f / float(a.head_dim));
+    return cudaGetLastError();
+}
 template <class T, int PT>
 cudaError_t launch_norm_rope(const NormRope& a, cudaStream_t stream) {
-    constexpr int U = 2, PER = kThreads / PT * U;
-    const int64_t qb = (int64_t(a.tokens) * a.q.heads + PER - 1) / PER, kb = (int64_t(a.tokens) * a.k.heads + PER - 1) / PER;
-    if (qb + kb > INT32_MAX) return cudaErrorInvalidValue;
-    norm_rope_kernel<T, PT, U><<<unsigned(qb + kb), kThreads, 0, stream>>>(a, int(qb));
-    return cudaGetLastError();
+    // few tokens: a thread a head, for the latency; else four heads a thread where there are as many
+    const int64_t heads = int64_t(a.tokens) * (a.q.heads + a.k.heads);
+    return std::max(a.q.heads, a.k.heads) >= 4 && heads * PT >= 148 * 2048 ? launch_norm_rope<T, PT, 4>(a, stream)
+                                                                           : launch_norm_rope<T, PT, 1>(a, stream);
 }
 template <class T>
 cudaError_t dispatch_norm_rope(const NormRope& a, cudaStream_t stream) {
@@ -179,12 +211,19 @@ cudaError_t dispatch_norm_rope(const NormRope& a, cudaStream_t stream) {
     return launch_norm_rope<T, 16>(a, stream);
 }
 
+template <class T, int PT, int U>
+cudaError_t launch_append(const PagedAppend& a, cudaStream_t stream) {
+    const int64_t units = (a.cache.kv_heads + U - 1) / U;
+    const int64_t per_seq = (int64_t(a.batch.max_chunk) * units + kThreads / PT - 1) / (kThreads / PT);
+    if (per_seq * a.batch.seqs > INT32_MAX || per_seq * (kThreads / PT) > INT32_MAX) return cudaErrorInvalidValue;
+    paged_append_kernel<T, PT, U><<<unsigned(per_seq * a.batch.seqs), kThreads, 0, stream>>>(a, FastDiv(uint32_t(per_seq)), FastDiv(uint32_t(units)),
+                                                                                               1.0f / float(a.cache.head_dim));
+    return cudaGetLastError();
+}
 template <class T, int PT>
 cudaError_t launch_append(const PagedAppend& a, cudaStream_t stream) {
-    const int64_t per_seq = (int64_t(a.batch.max_chunk) * a.cache.kv_heads + kThreads / PT - 1) / (kThreads / PT);
-    if (per_seq * a.batch.seqs > INT32_MAX) return cudaErrorInvalidValue;
-    paged_append_kernel<T, PT><<<unsigned(per_seq * a.batch.seqs), kThreads, 0, stream>>>(a, int(per_seq));
-    return cudaGetLastError();
+    return a.cache.kv_heads >= 2 && int64_t(a.batch.max_chunk) * a.batch.seqs * a.cache.kv_heads * PT >= 148 * 2048
+               ? launch_append<T, PT, 2>(a, stream) : launch_append<T, PT, 1>(a, stream);
 }
 
 }  // namespace

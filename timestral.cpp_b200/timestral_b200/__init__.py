@@ -137,10 +137,10 @@ SIGNATURES = {
     "tsb_test_fail_workspace_allocations": (C.c_int, [C.c_int32]),
     "tsb_test_device_reset": (C.c_int, []),
     "tsb_refine_static": (C.c_int, [C.c_void_p] * 6 + [C.c_int32] * 6 + [C.c_double, C.c_void_p, C.c_void_p]),
-    "tsb_norm_rope": (C.c_int, [C.POINTER(NormRopeArgs), C.c_void_p]),
-    "tsb_paged_append": (C.c_int, [C.POINTER(PagedAppendArgs), C.c_void_p]),
-    "tsb_paged_attention": (C.c_int, [C.POINTER(PagedAttentionArgs), C.c_void_p]),
-    "tsb_paged_attention_workspace": (C.c_size_t, [C.POINTER(PagedAttentionArgs)]),
+    "tsb_norm_rope": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "tsb_paged_append": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "tsb_paged_attention": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "tsb_paged_attention_workspace": (C.c_size_t, [C.c_void_p]),
 }
 
 

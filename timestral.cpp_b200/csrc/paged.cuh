@@ -127,6 +127,7 @@ __device__ __forceinline__ uint32_t unit_of(const PagedGrid& g, uint32_t unit, u
 struct PagedPlan {
     bool tiles = false;                 // paged_attention_tiles, else paged_attention_rows
     bool join = false;                  // rows: a block's teams share one problem
+    bool one = false;                   // rows: a tile holds every key
     int tile_rows = 0;
     int64_t row_tiles = 0, items = 0, whole = 0;
     int splits = 1;
@@ -219,15 +220,19 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
                       Pair<T>::down(f[6], f[7]));
 }
 
-// Keys [k0, k0 + 64) of the sequence whose bits are set (all of them without key_valid).
-__device__ __forceinline__ uint64_t valid_bits(const PagedAttention& a, int seq, int k0) {
-    if (!a.key_valid || k0 >= a.key_valid_positions) return ~0ull;
-    const uint32_t* w = a.key_valid + int64_t(seq) * a.key_valid_stride + (k0 >> 5);
+// Keys [k0, k0 + 32) of the sequence whose bits are set (all of them without key_valid).
+__device__ __forceinline__ uint32_t valid_word(const PagedAttention& a, int seq, int k0) {
     const int left = a.key_valid_positions - k0;
-    uint64_t m = w[0];
-    if (left > 32) m |= uint64_t(w[1]) << 32;
-    if (left < 64) m |= ~0ull << left;
-    return m;
+    if (left <= 0) return ~0u;
+    const uint32_t m = a.key_valid[int64_t(seq) * a.key_valid_stride + (k0 >> 5)];
+    return left < 32 ? m | ~0u << left : m;
+}
+// Bits [lo, hi] (inclusive, any ints) of the 32-bit word that starts at bit w0.
+__device__ __forceinline__ uint32_t range32(int lo, int hi, int w0) {
+    lo = max(lo - w0, 0);
+    hi = min(hi - w0, 31);
+    if (lo > hi) return 0u;
+    return (0xffffffffu >> (31 - hi)) & (0xffffffffu << lo);
 }
 
 }  // namespace tsb

@@ -34,11 +34,13 @@ namespace {
 constexpr int PR_THREADS = 128;
 constexpr float PR_RESCALE = 8.f;        // log2 of the largest probability kept unscaled
 
-template <int HD, int RG>
+// ONE: the tile holds every key of the problem (no window, max_length <= KT), so there is no ring.
+template <int HD, int RG, bool ONE>
 struct RowsLayout {
     static constexpr int TEAMS = 4 / RG;
-    static constexpr int KT = RG == 4 ? 64 : 32;            // keys of a tile: one or two copies a lane
-    static constexpr int STAGES = 3;
+    static constexpr int KT = ONE ? 96 : RG == 4 ? 64 : 32; // keys of a tile
+    static constexpr int BOX = KT == 64 ? 64 : 32;          // keys of one load at most
+    static constexpr int STAGES = ONE ? 1 : 3;
     static constexpr int HALF = KT * 128;                   // 64 values of the tile's keys
     static constexpr int TILE = HD / 64 * HALF;             // bytes of a tile of keys (or values)
     static constexpr int RING = STAGES * 2 * TILE;
@@ -116,13 +118,13 @@ __device__ __forceinline__ void quad_transpose(uint32_t (&v)[4]) {
     if (high) { v[0] = a; v[1] = b; } else { v[2] = a; v[3] = b; }
 }
 
-template <class T, int HD, int RG, int NR, bool JOIN>
-__global__ void __launch_bounds__(PR_THREADS)
+template <class T, int HD, int RG, int NR, bool JOIN, bool ONE>
+__global__ void __launch_bounds__(PR_THREADS, HD == 128 ? 1 : NR == 1 ? 5 : RG == 4 ? 3 : 4)
     paged_rows_kernel(const __grid_constant__ PageMaps maps, const PagedAttention a, const PagedGrid grid) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    using L = RowsLayout<HD, RG>;
-    constexpr int KT = L::KT, MK = KT / 16, KS = HD / 16, MD = HD / 16, WR = 8 * NR, MT = WR * RG;
+    using L = RowsLayout<HD, RG, ONE>;
+    constexpr int KT = L::KT, MK = KT / 16, NW = KT / 32, KS = HD / 16, MD = HD / 16, WR = 8 * NR, MT = WR * RG;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, rg = warp % RG, team = warp / RG;
 
     const uint32_t unit = blockIdx.x * (JOIN ? 1 : L::TEAMS) + (JOIN ? 0 : team);
@@ -159,7 +161,7 @@ __global__ void __launch_bounds__(PR_THREADS)
     team_sync<RG>(team);
 
     // The team's first warp loads: lane p the p-th page that the tile touches.
-    const int slots = 1 << a.cache.page_shift, box = min(slots, KT);
+    const int slots = 1 << a.cache.page_shift, box = min(slots, L::BOX);
     const int* table = a.cache.table + int64_t(t.seq) * a.cache.table_stride;
     auto page_of = [&](int tile) {
         const int key = tile * KT + lane * box;
@@ -187,9 +189,9 @@ __global__ void __launch_bounds__(PR_THREADS)
     };
     int page = page_of(first);
 #pragma unroll
-    for (int s = 0; s < L::STAGES - 1; ++s) {
+    for (int s = 0; s < (ONE ? 1 : L::STAGES - 1); ++s) {
         if (first + s * STEP < last) load_tile(first + s * STEP, s, page);
-        page = page_of(first + (s + 1) * STEP);
+        if (!ONE) page = page_of(first + (s + 1) * STEP);
     }
 
     // Fragments: of a query row this lane holds row lane / 4 (+ 8 n), of a score or weighted value the
@@ -197,6 +199,9 @@ __global__ void __launch_bounds__(PR_THREADS)
     // every key).
     int pos[NR][2];
     uint32_t qf[KS][NR][2];
+    // with a negative scale the queries' signs turn, so that the largest product has the largest score
+    const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+    const float scale = fabsf(a.scale_log2);
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
 #pragma unroll
@@ -209,8 +214,8 @@ __global__ void __launch_bounds__(PR_THREADS)
                                                               (t.kvh * a.group + m - tok * a.group) * a.q.head) + (lane & 3);
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-            qf[k][n][0] = r < t.rows ? p[k * 8] : 0u;
-            qf[k][n][1] = r < t.rows ? p[k * 8 + 4] : 0u;
+            qf[k][n][0] = r < t.rows ? p[k * 8] ^ flip : 0u;
+            qf[k][n][1] = r < t.rows ? p[k * 8 + 4] ^ flip : 0u;
         }
     }
     float o[MD][NR][4];
@@ -228,22 +233,28 @@ __global__ void __launch_bounds__(PR_THREADS)
         if (!expired && !mbar_wait(&full[st], phase)) { record_error(a.err, kDevTimeoutAttn); expired = true; }
         const int k0 = tile * KT;
         uint8_t* const tk = ring + st * 2 * L::TILE;
-        uint64_t valid = ~0ull;
-        if (a.key_valid) valid = valid_bits(a, t.seq, k0 & ~63) >> (k0 & 63);
-        const bool whole = KT == 64 ? valid == ~0ull : uint32_t(valid) == ~0u;     // every bit is set
+        uint32_t valid[NW];
+        bool whole = true;                          // every bit is set
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            valid[w] = ~0u;
+            if (a.key_valid) { valid[w] = valid_word(a, t.seq, k0 + w * 32); whole = whole && valid[w] == ~0u; }
+        }
         if (k0 < t.lo || k0 + KT > t.hi || !whole) {
             // values of keys that no row sees: zeros instead of what stands there
-            for (int r = threadIdx.x % (32 * RG); r < KT; r += 32 * RG) {
-                const int key = k0 + r;
-                if (key >= t.lo && key < t.hi && (((valid >> r) & 1) || (a.self_visible && key >= t.base))) continue;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) {
+                if (NW % RG == 0 ? w % RG != rg : rg != 0) continue;       // a warp a word, or the first all of them
+                const int r = w * 32 + lane, key = k0 + r;
+                if (key >= t.lo && key < t.hi && (((valid[w] >> lane) & 1) || (a.self_visible && key >= t.base))) continue;
 #pragma unroll
                 for (int c = 0; c < HD / 8; ++c)
-                    *reinterpret_cast<uint4*>(tk + L::TILE + (c / 8) * L::HALF + r * 128 + (((c + r) & 7) << 4)) = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4*>(tk + L::TILE + (c / 8) * L::HALF + r * 128 + (((c + lane) & 7) << 4)) = make_uint4(0, 0, 0, 0);
             }
             fence_proxy_async();                    // before a later load into the stage
         }
         team_sync<RG>(team);                        // zeros are written; the stage read last is free
-        {
+        if constexpr (!ONE) {
             const int nx = tile + (L::STAGES - 1) * STEP, ns = st == 0 ? L::STAGES - 1 : st - 1;
             if (nx < last) load_tile(nx, ns, page);
             page = page_of(nx + STEP);
@@ -256,41 +267,40 @@ __global__ void __launch_bounds__(PR_THREADS)
 #pragma unroll
             for (int n = 0; n < NR; ++n) sc[i][n][0] = sc[i][n][1] = sc[i][n][2] = sc[i][n][3] = 0.f;
         const uint32_t ka = sk + (lane & 15) * 128, kx = ((lane & 7) ^ (lane >> 4)) << 4;
+        // (16 keys behind the last that the rows see cost nothing; the first 16 of a tile are always tried)
+        const int here = ONE ? (t.hi - k0 + 15) / 16 : MK;
 #pragma unroll
-        for (int k = 0; k < KS; ++k)
+        for (int i = 0; i < MK; ++i) {
+            if (ONE && i >= here) break;
 #pragma unroll
-            for (int i = 0; i < MK; ++i) {
+            for (int k = 0; k < KS; ++k) {
                 uint32_t f[4];
                 ldsm4(ka + (k / 4) * L::HALF + i * 16 * 128 + (kx ^ ((k % 4) << 5)), f);
 #pragma unroll
                 for (int n = 0; n < NR; ++n) mma16816<T>(sc[i][n], f, qf[k][n][0], qf[k][n][1]);
             }
+        }
         // every row of the tile sees every key of it: no per-key masks
         const bool all = k0 + KT - 1 <= t.base + t_first && (a.window == 0 || k0 > t.base + t_last - a.window) && whole;
+        if (!all) {
 #pragma unroll
-        for (int n = 0; n < NR; ++n)
+            for (int n = 0; n < NR; ++n)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                // bit 8 j of the row's keys, from this lane's first (lane / 4) on
-                uint64_t see = 0;
-                if (!all) {
-                    const int p = pos[n][e] - k0;
-                    if (p >= 0) {
-                        see = valid & (p >= 63 ? ~0ull : (2ull << p) - 1);
-                        if (a.window && p >= a.window) see &= p - a.window >= 63 ? 0ull : ~((2ull << (p - a.window)) - 1);
-                        if (a.self_visible && p < 64) see |= 1ull << p;
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int w = 0; w < NW; ++w) {
+                        // bit 8 j of the row's keys of this word, from this lane's first (lane / 4) on
+                        const int w0 = k0 + w * 32, p = pos[n][e];
+                        uint32_t see = valid[w] & range32(a.window ? p - a.window + 1 : 0, p, w0);
+                        if (a.self_visible) see |= range32(p, p, w0);
+                        see >>= lane >> 2;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            float& x = sc[w * 2 + j / 2][n][2 * (j & 1) + e];
+                            if (!((see >> (8 * j)) & 1)) x = -INFINITY;
+                        }
                     }
-                    see >>= lane >> 2;
-                }
-#pragma unroll
-                for (int i = 0; i < MK; ++i)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        float& x = sc[i][n][2 * h + e];
-                        x *= a.scale_log2;
-                        if (!all && !((see >> (i * 16 + h * 8)) & 1)) x = -INFINITY;
-                    }
-            }
+        }
         // The reference maximum of a row moves only when a score passes it by more than 2^8: then the
         // sums are scaled down, which most tiles spare.
         float m[NR][2];
@@ -304,7 +314,7 @@ __global__ void __launch_bounds__(PR_THREADS)
                 for (int i = 1; i < MK; ++i) x = fmaxf(x, fmaxf(sc[i][n][e], sc[i][n][2 + e]));
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16)) * scale;
                 m[n][e] = x;
                 up |= x > mx[n][e] + PR_RESCALE;
             }
@@ -328,14 +338,15 @@ __global__ void __launch_bounds__(PR_THREADS)
                 const float ref = mx[n][e] == -INFINITY ? 0.f : mx[n][e];
 #pragma unroll
                 for (int i = 0; i < MK; ++i) {
-                    sc[i][n][e] = exp2_ftz(sc[i][n][e] - ref);
-                    sc[i][n][2 + e] = exp2_ftz(sc[i][n][2 + e] - ref);
+                    sc[i][n][e] = exp2_ftz(fmaf(sc[i][n][e], scale, -ref));
+                    sc[i][n][2 + e] = exp2_ftz(fmaf(sc[i][n][2 + e], scale, -ref));
                     sum[n][e] += sc[i][n][e] + sc[i][n][2 + e];
                 }
             }
         const uint32_t va = sv + ((lane & 7) + ((lane >> 4) << 3)) * 128, vx = ((lane & 7) ^ ((lane >> 3) & 1)) << 4;
 #pragma unroll
         for (int i = 0; i < MK; ++i) {
+            if (ONE && i >= here) break;
             uint32_t p[NR][2];
 #pragma unroll
             for (int n = 0; n < NR; ++n) {
@@ -529,32 +540,38 @@ int rows_of_team(const PagedAttention& a) {
     return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
 }
 
-template <class T, int HD, int RG, int NR, bool JOIN>
+template <class T, int HD, int RG, int NR, bool JOIN, bool ONE>
 cudaError_t launch_rows(const PagedAttention& a, const PagedGrid& grid, cudaStream_t stream) {
-    using L = RowsLayout<HD, RG>;
+    using L = RowsLayout<HD, RG, ONE>;
     static KernelSetup configured;
     int dev = 0;
     cudaGetDevice(&dev);
     unsigned long long key = 0;
     if (configured.needed(dev, &key)) {
-        const cudaError_t e = cudaFuncSetAttribute(paged_rows_kernel<T, HD, RG, NR, JOIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
+        const cudaError_t e = cudaFuncSetAttribute(paged_rows_kernel<T, HD, RG, NR, JOIN, ONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
         if (e != cudaSuccess) return e;
         configured.done(dev, key);
     }
     PageMaps maps;
-    if (!page_maps(&maps, a.cache, std::is_same<T, __nv_bfloat16>::value, L::KT)) return cudaErrorInvalidValue;
+    if (!page_maps(&maps, a.cache, std::is_same<T, __nv_bfloat16>::value, L::BOX)) return cudaErrorInvalidValue;
     const unsigned blocks = JOIN ? grid.units : (grid.units + L::TEAMS - 1) / L::TEAMS;
-    paged_rows_kernel<T, HD, RG, NR, JOIN><<<blocks, PR_THREADS, L::SMEM, stream>>>(maps, a, grid);
+    paged_rows_kernel<T, HD, RG, NR, JOIN, ONE><<<blocks, PR_THREADS, L::SMEM, stream>>>(maps, a, grid);
     return cudaGetLastError();
 }
 template <class T, int HD>
 cudaError_t dispatch_rows(const PagedAttention& a, const PagedGrid& grid, const PagedPlan& plan, cudaStream_t stream) {
+    if (plan.one) switch (plan.tile_rows) {
+        case 8: return launch_rows<T, HD, 1, 1, false, true>(a, grid, stream);
+        case 16: return launch_rows<T, HD, 2, 1, false, true>(a, grid, stream);
+        case 32: return launch_rows<T, HD, 4, 1, false, true>(a, grid, stream);
+        default: return launch_rows<T, HD, 4, 2, false, true>(a, grid, stream);
+    }
     const bool join = plan.join;
     switch (plan.tile_rows) {
-        case 8: return join ? launch_rows<T, HD, 1, 1, true>(a, grid, stream) : launch_rows<T, HD, 1, 1, false>(a, grid, stream);
-        case 16: return join ? launch_rows<T, HD, 1, 2, true>(a, grid, stream) : launch_rows<T, HD, 1, 2, false>(a, grid, stream);
-        case 32: return join ? launch_rows<T, HD, 2, 2, true>(a, grid, stream) : launch_rows<T, HD, 2, 2, false>(a, grid, stream);
-        default: return launch_rows<T, HD, 4, 2, false>(a, grid, stream);     // one team
+        case 8: return join ? launch_rows<T, HD, 1, 1, true, false>(a, grid, stream) : launch_rows<T, HD, 1, 1, false, false>(a, grid, stream);
+        case 16: return join ? launch_rows<T, HD, 1, 2, true, false>(a, grid, stream) : launch_rows<T, HD, 1, 2, false, false>(a, grid, stream);
+        case 32: return join ? launch_rows<T, HD, 2, 2, true, false>(a, grid, stream) : launch_rows<T, HD, 2, 2, false, false>(a, grid, stream);
+        default: return launch_rows<T, HD, 4, 2, false, false>(a, grid, stream);     // one team
     }
 }
 
@@ -628,6 +645,7 @@ PagedPlan paged_plan(const PagedAttention& a) {
             if (cost < best) { best = cost; p.splits = s; }
         }
     } else {
+        p.one = !a.window && a.batch.max_length <= 96;
         p.join = rows <= 32 && keys > 256;
         p.splits = int(std::max<int64_t>(1, std::min<int64_t>({p.items >= sms ? (4 * sms + p.items - 1) / p.items : sms / p.items, (keys + 255) / 256, 256})));
     }

@@ -77,14 +77,6 @@ __device__ __forceinline__ bool role_wait_warp(uint64_t* bar, uint32_t parity, v
     return __all_sync(0xffffffffu, ok);
 }
 
-// Bits [lo, hi] (inclusive, any ints) of the 32-bit word that starts at bit w0.
-__device__ __forceinline__ uint32_t range32(int lo, int hi, int w0) {
-    lo = max(lo - w0, 0);
-    hi = min(hi - w0, 31);
-    if (lo > hi) return 0u;
-    return (0xffffffffu >> (31 - hi)) & (0xffffffffu << lo);
-}
-
 __device__ __forceinline__ uint64_t desc_of(uint32_t lo, uint32_t hi) {
     uint64_t d;
     asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
@@ -317,16 +309,20 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
         bool ok = true;
         for (int j = 0; j < ngg; ++j) {
             const int k0 = (first + j) * PT_KT;
-            uint64_t v01 = ~0ull, v23 = ~0ull;
-            if (a.key_valid) { v01 = valid_bits(a, seq, k0); v23 = valid_bits(a, seq, k0 + 64); }
-            const bool dead_keys = k0 < lo || k0 + PT_KT > hi || (v01 & v23) != ~0ull;
-            const bool plain = k0 + PT_KT - 1 <= pos_first && (!a.window || k0 > pos_last - a.window) && (v01 & v23) == ~0ull;
+            uint32_t vw[4] = {~0u, ~0u, ~0u, ~0u};
+            if (a.key_valid)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) vw[w] = valid_word(a, seq, k0 + w * 32);
+            const bool whole = (vw[0] & vw[1] & vw[2] & vw[3]) == ~0u;
+            const bool dead_keys = k0 < lo || k0 + PT_KT > hi || !whole;
+            const bool plain = k0 + PT_KT - 1 <= pos_first && (!a.window || k0 > pos_last - a.window) && whole;
             if (dead_keys && g == (j < ng[0] ? 0 : 1)) {
                 // values of keys that no row of the block sees: zeros instead of what stands there
                 const int i = 2 * j + 1;
                 if (!(ok = role_wait_warp(&bars->full[i % L::STAGES], (i / L::STAGES) & 1, abort, a.err))) break;
                 const int key = k0 + t;
-                const bool valid = ((t < 64 ? v01 >> t : v23 >> (t - 64)) & 1) || (a.self_visible && key >= base);
+                const uint32_t word = t < 64 ? (t < 32 ? vw[0] : vw[1]) : (t < 96 ? vw[2] : vw[3]);
+                const bool valid = ((word >> lane) & 1) || (a.self_visible && key >= base);
                 if (key < lo || key >= hi || !valid) {
                     uint8_t* v = ring + i % L::STAGES * L::SLOT + t * 128;
 #pragma unroll
@@ -341,7 +337,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             // a quarter of the scores is loaded while the maximum of the one before is taken
             uint32_t s[4][32];
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            const uint32_t vw[4] = {uint32_t(v01), uint32_t(v01 >> 32), uint32_t(v23), uint32_t(v23 >> 32)};
             tmem_ld32(ts, s[0]);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {

@@ -144,12 +144,13 @@ __global__ void __launch_bounds__(PR_THREADS, HD == 128 ? 1 : NR == 1 ? 5 : RG =
     t.base = q.len - q.n;
     const int t_first = int(grid.group.div(t.m0)), t_last = int(grid.group.div(t.m0 + t.rows - 1));
     t.hi = t.base + t_last + 1;
-    t.lo = a.window ? max(0, t.base + t_first - a.window + 1) : 0;
+    t.lo = !ONE && a.window ? max(0, t.base + t_first - a.window + 1) : 0;
     // this item's share of the tiles, and of those this team's
-    const int tile0 = t.lo / KT, tiles = (t.hi + KT - 1) / KT - tile0;
+    const int tile0 = ONE ? 0 : t.lo / KT, tiles = ONE ? 1 : (t.hi + KT - 1) / KT - tile0;
     const int share = splits > 1 ? int(grid.splits.div(tiles + splits - 1)) : tiles;
     constexpr int STEP = JOIN ? L::TEAMS : 1;
-    const int first = tile0 + int(split) * share + (JOIN ? team : 0), last = min(tile0 + (int(split) + 1) * share, tile0 + tiles);
+    const int first = ONE ? 0 : tile0 + int(split) * share + (JOIN ? team : 0);
+    const int last = ONE ? 1 : min(tile0 + (int(split) + 1) * share, tile0 + tiles);
 
     uint8_t* ring = smem + team * L::RING;
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::TEAMS * L::RING) + team * L::STAGES;
@@ -218,6 +219,19 @@ __global__ void __launch_bounds__(PR_THREADS, HD == 128 ? 1 : NR == 1 ? 5 : RG =
             qf[k][n][1] = r < t.rows ? p[k * 8 + 4] ^ flip : 0u;
         }
     }
+    // A short problem's gate and key bits are on their way while its keys are.
+    uint32_t gv[ONE ? NR : 1][ONE ? HD / 8 : 1];
+    if constexpr (ONE) {
+        if (a.gate.data)
+#pragma unroll
+            for (int n = 0; n < NR; ++n) {
+                const int r = rg * WR + n * 8 + lane / 4, m = t.m0 + r, tok = int(grid.group.div(m));
+                const T* gate = static_cast<const T*>(a.gate.data) + (t.start + tok) * a.gate.token + (t.kvh * a.group + m - tok * a.group) * a.gate.head;
+#pragma unroll
+                for (int b = 0; b < HD / 8; ++b)
+                    gv[n][b] = r < t.rows ? *reinterpret_cast<const uint32_t*>(gate + b * 8 + (lane & 3) * 2) : 0u;
+            }
+    }
     float o[MD][NR][4];
 #pragma unroll
     for (int d = 0; d < MD; ++d)
@@ -230,16 +244,15 @@ __global__ void __launch_bounds__(PR_THREADS, HD == 128 ? 1 : NR == 1 ? 5 : RG =
     int st = 0, phase = 0;
     bool expired = false;       // after an expired wait the team goes on, without waits, to meet its barriers
     for (int tile = first; tile < last; tile += STEP) {
-        if (!expired && !mbar_wait(&full[st], phase)) { record_error(a.err, kDevTimeoutAttn); expired = true; }
-        const int k0 = tile * KT;
-        uint8_t* const tk = ring + st * 2 * L::TILE;
+        const int k0 = ONE ? 0 : tile * KT;
         uint32_t valid[NW];
         bool whole = true;                          // every bit is set
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            valid[w] = ~0u;
-            if (a.key_valid) { valid[w] = valid_word(a, t.seq, k0 + w * 32); whole = whole && valid[w] == ~0u; }
-        }
+        for (int w = 0; w < NW; ++w) valid[w] = a.key_valid ? valid_word(a, t.seq, k0 + w * 32) : ~0u;
+        if (!expired && !mbar_wait(&full[st], phase)) { record_error(a.err, kDevTimeoutAttn); expired = true; }
+        uint8_t* const tk = ring + st * 2 * L::TILE;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) whole = whole && valid[w] == ~0u;
         if (k0 < t.lo || k0 + KT > t.hi || !whole) {
             // values of keys that no row sees: zeros instead of what stands there
 #pragma unroll
@@ -290,9 +303,10 @@ __global__ void __launch_bounds__(PR_THREADS, HD == 128 ? 1 : NR == 1 ? 5 : RG =
 #pragma unroll
                     for (int w = 0; w < NW; ++w) {
                         // bit 8 j of the row's keys of this word, from this lane's first (lane / 4) on
-                        const int w0 = k0 + w * 32, p = pos[n][e];
-                        uint32_t see = valid[w] & range32(a.window ? p - a.window + 1 : 0, p, w0);
-                        if (a.self_visible) see |= range32(p, p, w0);
+                        const int p = pos[n][e] - k0 - w * 32;                 // the row's own key, counted from the word
+                        uint32_t see = p < 0 ? 0u : p >= 31 ? valid[w] : valid[w] & ((2u << p) - 1);
+                        if (!ONE && a.window) see &= range32(p - a.window + 1, 31, 0);
+                        if (a.self_visible && p >= 0 && p < 32) see |= 1u << p;
                         see >>= lane >> 2;
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
@@ -318,7 +332,10 @@ __global__ void __launch_bounds__(PR_THREADS, HD == 128 ? 1 : NR == 1 ? 5 : RG =
                 m[n][e] = x;
                 up |= x > mx[n][e] + PR_RESCALE;
             }
-        if (__any_sync(0xffffffffu, up)) {
+        if constexpr (ONE) {
+#pragma unroll
+            for (int n = 0; n < NR; ++n) { mx[n][0] = m[n][0]; mx[n][1] = m[n][1]; }
+        } else if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
             for (int n = 0; n < NR; ++n)
 #pragma unroll
@@ -411,7 +428,9 @@ __global__ void __launch_bounds__(PR_THREADS, HD == 128 ? 1 : NR == 1 ? 5 : RG =
                 for (int i = 0; i < 4; ++i) {
                     float x = o[(b + i) / 2][n][((b + i) & 1) * 2] * inv[0], y = o[(b + i) / 2][n][((b + i) & 1) * 2 + 1] * inv[1];
                     if (a.gate.data) {
-                        const uint32_t g = there ? *reinterpret_cast<const uint32_t*>(gate + (b + i) * 8 + (lane & 3) * 2) : 0u;
+                        uint32_t g;
+                        if constexpr (ONE) g = gv[n][b + i];
+                        else g = there ? *reinterpret_cast<const uint32_t*>(gate + (b + i) * 8 + (lane & 3) * 2) : 0u;
                         const float2 gf = Pair<T>::up(turn8x8(g));
                         x *= gf.x;
                         y *= gf.y;

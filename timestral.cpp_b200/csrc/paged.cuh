@@ -102,6 +102,7 @@ struct PagedAttention {
 struct PagedGrid {
     FastDiv splits, heads, seqs, group;
     uint32_t items = 0, whole = 0, units = 0, row_tiles = 0;
+    uint32_t one_keys = 0;              // rows, a tile for all keys: the tile's keys
 };
 struct PagedItem {
     int row_tile, kvh, seq;

@@ -34,17 +34,19 @@ namespace {
 constexpr int PR_THREADS = 128;
 constexpr float PR_RESCALE = 8.f;        // log2 of the largest probability kept unscaled
 
-// ONE: the tile holds every key of the problem (no window, max_length <= KT), so there is no ring.
+// ONE: the tile holds every key of the problem (no window, max_length <= KT), so there is no ring, and
+// the tile takes no more shared memory than max_length rounded up to 16 keys, for more blocks an SM.
 template <int HD, int RG, bool ONE>
 struct RowsLayout {
     static constexpr int TEAMS = 4 / RG;
     static constexpr int KT = ONE ? 96 : RG == 4 ? 64 : 32; // keys of a tile
-    static constexpr int BOX = KT == 64 ? 64 : 32;          // keys of one load at most
+    static constexpr int BOX = ONE ? 16 : KT;         // keys of one load at most
     static constexpr int STAGES = ONE ? 1 : 3;
     static constexpr int HALF = KT * 128;                   // 64 values of the tile's keys
     static constexpr int TILE = HD / 64 * HALF;             // bytes of a tile of keys (or values)
     static constexpr int RING = STAGES * 2 * TILE;
     static constexpr int SMEM = 1024 + TEAMS * RING + TEAMS * STAGES * 8;
+    static int smem(int keys) { return ONE ? 1024 + TEAMS * (2 * HD / 64 * keys * 128 + 8) : SMEM; }
     static_assert(SMEM >= 4 * 16 * HD * 4 + 4 * 16 * 8, "the joined rows reuse the rings");
 };
 
@@ -152,8 +154,9 @@ __global__ void __launch_bounds__(PR_THREADS, HD == 128 ? 1 : NR == 1 ? 5 : RG =
     const int first = ONE ? 0 : tile0 + int(split) * share + (JOIN ? team : 0);
     const int last = ONE ? 1 : min(tile0 + (int(split) + 1) * share, tile0 + tiles);
 
-    uint8_t* ring = smem + team * L::RING;
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::TEAMS * L::RING) + team * L::STAGES;
+    const int half = ONE ? int(grid.one_keys) * 128 : L::HALF, tile_bytes = ONE ? HD / 64 * half : L::TILE;
+    uint8_t* ring = smem + team * (L::STAGES * 2 * tile_bytes);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::TEAMS * L::STAGES * 2 * tile_bytes) + team * L::STAGES;
     if (rg == 0 && lane == 0) {
         for (int s = 0; s < L::STAGES; ++s) mbar_init(&full[s], 1);
         mbar_fence_init();
@@ -179,11 +182,11 @@ __global__ void __launch_bounds__(PR_THREADS, HD == 128 ? 1 : NR == 1 ? 5 : RG =
         __syncwarp();
         if (page >= 0) {
             const int slot = (tile * KT + lane * box) & (slots - 1);
-            uint8_t* dst = ring + stage * 2 * L::TILE + lane * box * 128;
+            uint8_t* dst = ring + stage * 2 * tile_bytes + lane * box * 128;
 #pragma unroll
             for (int h = 0; h < HD / 64; ++h) {
-                load_page(dst + h * L::HALF, maps.k, &full[stage], h * 64, slot, t.kvh, page);
-                load_page(dst + L::TILE + h * L::HALF, maps.v, &full[stage], h * 64, slot, t.kvh, page);
+                load_page(dst + h * half, maps.k, &full[stage], h * 64, slot, t.kvh, page);
+                load_page(dst + tile_bytes + h * half, maps.v, &full[stage], h * 64, slot, t.kvh, page);
             }
         }
         __syncwarp();
@@ -250,7 +253,7 @@ __global__ void __launch_bounds__(PR_THREADS, HD == 128 ? 1 : NR == 1 ? 5 : RG =
 #pragma unroll
         for (int w = 0; w < NW; ++w) valid[w] = a.key_valid ? valid_word(a, t.seq, k0 + w * 32) : ~0u;
         if (!expired && !mbar_wait(&full[st], phase)) { record_error(a.err, kDevTimeoutAttn); expired = true; }
-        uint8_t* const tk = ring + st * 2 * L::TILE;
+        uint8_t* const tk = ring + st * 2 * tile_bytes;
 #pragma unroll
         for (int w = 0; w < NW; ++w) whole = whole && valid[w] == ~0u;
         if (k0 < t.lo || k0 + KT > t.hi || !whole) {
@@ -259,10 +262,11 @@ __global__ void __launch_bounds__(PR_THREADS, HD == 128 ? 1 : NR == 1 ? 5 : RG =
             for (int w = 0; w < NW; ++w) {
                 if (NW % RG == 0 ? w % RG != rg : rg != 0) continue;       // a warp a word, or the first all of them
                 const int r = w * 32 + lane, key = k0 + r;
+                if (ONE && r >= int(grid.one_keys)) continue;
                 if (key >= t.lo && key < t.hi && (((valid[w] >> lane) & 1) || (a.self_visible && key >= t.base))) continue;
 #pragma unroll
                 for (int c = 0; c < HD / 8; ++c)
-                    *reinterpret_cast<uint4*>(tk + L::TILE + (c / 8) * L::HALF + r * 128 + (((c + lane) & 7) << 4)) = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4*>(tk + tile_bytes + (c / 8) * half + r * 128 + (((c + lane) & 7) << 4)) = make_uint4(0, 0, 0, 0);
             }
             fence_proxy_async();                    // before a later load into the stage
         }
@@ -272,7 +276,7 @@ __global__ void __launch_bounds__(PR_THREADS, HD == 128 ? 1 : NR == 1 ? 5 : RG =
             if (nx < last) load_tile(nx, ns, page);
             page = page_of(nx + STEP);
         }
-        const uint32_t sk = smem_u32(tk), sv = sk + L::TILE;
+        const uint32_t sk = smem_u32(tk), sv = sk + tile_bytes;
         if (++st == L::STAGES) { st = 0; phase ^= 1; }
         float sc[MK][NR][4];
 #pragma unroll
@@ -288,7 +292,7 @@ __global__ void __launch_bounds__(PR_THREADS, HD == 128 ? 1 : NR == 1 ? 5 : RG =
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
                 uint32_t f[4];
-                ldsm4(ka + (k / 4) * L::HALF + i * 16 * 128 + (kx ^ ((k % 4) << 5)), f);
+                ldsm4(ka + (k / 4) * half + i * 16 * 128 + (kx ^ ((k % 4) << 5)), f);
 #pragma unroll
                 for (int n = 0; n < NR; ++n) mma16816<T>(sc[i][n], f, qf[k][n][0], qf[k][n][1]);
             }
@@ -373,7 +377,7 @@ __global__ void __launch_bounds__(PR_THREADS, HD == 128 ? 1 : NR == 1 ? 5 : RG =
 #pragma unroll
             for (int d = 0; d < MD; ++d) {
                 uint32_t f[4];
-                ldsm4_t(va + (d / 4) * L::HALF + i * 16 * 128 + (vx ^ ((d % 4) << 5)), f);
+                ldsm4_t(va + (d / 4) * half + i * 16 * 128 + (vx ^ ((d % 4) << 5)), f);
 #pragma unroll
                 for (int n = 0; n < NR; ++n) mma16816<T>(o[d][n], f, p[n][0], p[n][1]);
             }
@@ -574,7 +578,7 @@ cudaError_t launch_rows(const PagedAttention& a, const PagedGrid& grid, cudaStre
     PageMaps maps;
     if (!page_maps(&maps, a.cache, std::is_same<T, __nv_bfloat16>::value, L::BOX)) return cudaErrorInvalidValue;
     const unsigned blocks = JOIN ? grid.units : (grid.units + L::TEAMS - 1) / L::TEAMS;
-    paged_rows_kernel<T, HD, RG, NR, JOIN, ONE><<<blocks, PR_THREADS, L::SMEM, stream>>>(maps, a, grid);
+    paged_rows_kernel<T, HD, RG, NR, JOIN, ONE><<<blocks, PR_THREADS, L::smem(int(grid.one_keys)), stream>>>(maps, a, grid);
     return cudaGetLastError();
 }
 template <class T, int HD>
@@ -685,6 +689,7 @@ cudaError_t paged_attention(const PagedAttention& a, bool bf16, cudaStream_t str
     g.whole = uint32_t(whole);
     g.units = uint32_t(units);
     g.row_tiles = uint32_t(p.row_tiles);
+    g.one_keys = uint32_t(std::max(16, (a.batch.max_length + 15) / 16 * 16));
     if (a.cache.head_dim == 64) return bf16 ? dispatch<__nv_bfloat16, 64>(a, p, g, stream) : dispatch<__half, 64>(a, p, g, stream);
     return bf16 ? dispatch<__nv_bfloat16, 128>(a, p, g, stream) : dispatch<__half, 128>(a, p, g, stream);
 }

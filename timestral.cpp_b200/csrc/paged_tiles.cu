@@ -122,6 +122,27 @@ __device__ __forceinline__ void exp2_poly(F2 x, float& r0, float& r1) {
     r1 = __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23));
 }
 
+// MMAs and commits of a converged warp, issued by its elected lane: with the warp together the
+// descriptors stay in uniform registers, where a branch for one lane moves them there for each MMA.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n elect.sync _|e, 0xffffffff;\n"
+        " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(accumulate))
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n elect.sync _|e, 0xffffffff;\n"
+        " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(uint32_t(accumulate))
+        : "memory");
+}
+__device__ __forceinline__ void mma_commit_warp(uint64_t* bar) {
+    asm volatile(
+        "{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
+        " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar))
+        : "memory");
+}
+
 template <class T, int HD>
 __global__ void __launch_bounds__(PT_THREADS, 1)
     paged_tiles_kernel(const __grid_constant__ PageMaps maps, const PagedAttention a, const PagedGrid grid) {
@@ -131,7 +152,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     uint8_t* ring = qbuf + 2 * L::SLOT;
     TilesBars* bars = reinterpret_cast<TilesBars*>(ring + L::STAGES * L::SLOT);
     volatile int* abort = &bars->abort;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;    // (known to be uniform)
 
     uint32_t split;
     int splits;
@@ -218,7 +239,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                 __syncwarp();
             }
         } else if (warp == 8) {
-            if (lane == 0) {
+            {
                 // Few instructions between the MMAs, which they would hold up: descriptors differ from the ring
                 // slot's in their low word alone, by constants.
                 constexpr uint32_t bf = std::is_same<T, __nv_bfloat16>::value ? kIdescBf16 : 0u;
@@ -228,26 +249,26 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                 const uint32_t hi = uint32_t(dq >> 32), hi_v = uint32_t(dv >> 32), lo_q = uint32_t(dq), lo_r = uint32_t(dr), lo_v = uint32_t(dv);
                 constexpr uint32_t SLOT16 = L::SLOT >> 4;
                 int slot = 0, phase = 0;                                // of the next tile in the ring
-                auto full = [&]() { return role_wait(&bars->full[slot], phase, abort, a.err); };
+                auto full = [&]() { return role_wait_warp(&bars->full[slot], phase, abort, a.err); };
                 auto next = [&]() { if (++slot == L::STAGES) { slot = 0; phase ^= 1; } };
                 auto scores = [&](int gg) {                             // S_gg = Q_gg K of the ring's next tile
                     const uint32_t q = lo_q + gg * SLOT16, k = lo_r + slot * SLOT16;
 #pragma unroll
                     for (int i = 0; i < HD / 16; ++i) {
                         const uint32_t off = (i / 4) * (L::HALF >> 4) + (i % 4) * 2;
-                        mma_f16(tbase + gg * 128, desc_of(q + off, hi), desc_of(k + off, hi), id_qk, i > 0);
+                        mma_ss(tbase + gg * 128, desc_of(q + off, hi), desc_of(k + off, hi), id_qk, i > 0);
                     }
-                    mma_commit(&bars->s_full[gg]);
+                    mma_commit_warp(&bars->s_full[gg]);
                 };
                 bool ok = full();
 #pragma unroll
                 for (int gg = 0; gg < 2; ++gg)
                     if (ok && ng[gg] > 0) {
-                        ok = role_wait(&bars->q_ready[gg], 0, abort, a.err);
+                        ok = role_wait_warp(&bars->q_ready[gg], 0, abort, a.err);
                         tc_fence_after();
                         if (ok) scores(gg);
                     }
-                if (ok) mma_commit(&bars->empty[0]);
+                if (ok) mma_commit_warp(&bars->empty[0]);
                 next();
                 for (int j = 0; j < nt && ok; ++j) {
                     ok = full();
@@ -261,20 +282,20 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                             // the first half of the probabilities is multiplied while the second is made
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
-                                if (ok) ok = role_wait(&bars->p_ready[gg][h], j & 1, abort, a.err);
+                                if (ok) ok = role_wait_warp(&bars->p_ready[gg][h], j & 1, abort, a.err);
                                 tc_fence_after();
                                 if (!ok) break;
 #pragma unroll
                                 for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
-                                    mma_f16_ts(tbase + PT_O_COL + gg * 128, tbase + gg * 128 + kk * 8, desc_of(v + kk * 128, hi_v), id_pv,
+                                    mma_ts(tbase + PT_O_COL + gg * 128, tbase + gg * 128 + kk * 8, desc_of(v + kk * 128, hi_v), id_pv,
                                                j > 0 || kk > 0);
                             }
                             if (ok && j + 1 < ng[gg]) scores(gg);
-                            if (ok && j + 1 == ng[gg]) mma_commit(&bars->o_full[gg]);
+                            if (ok && j + 1 == ng[gg]) mma_commit_warp(&bars->o_full[gg]);
                         }
-                        if (ok && gg == 1) mma_commit(&bars->empty[vslot]);
+                        if (ok && gg == 1) mma_commit_warp(&bars->empty[vslot]);
                     }
-                    if (ok && j + 1 < nt) { mma_commit(&bars->empty[slot]); next(); }
+                    if (ok && j + 1 < nt) { mma_commit_warp(&bars->empty[slot]); next(); }
                 }
             }
             __syncwarp();

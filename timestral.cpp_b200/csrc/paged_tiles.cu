@@ -31,8 +31,6 @@ constexpr int PT_LAUNCH_REGS = 168, PT_SOFTMAX_REGS = 216, PT_OTHER_REGS = 72;
 static_assert(256 * PT_SOFTMAX_REGS + 128 * PT_OTHER_REGS <= PT_THREADS * PT_LAUNCH_REGS);
 constexpr int PT_KT = 128;
 constexpr uint32_t PT_TMEM = 512, PT_O_COL = 256;
-// Of every PT_POLY_OF pairs of probabilities so many come from exp2_poly.
-constexpr int PT_POLY_OF = 8, PT_POLY_64 = 0, PT_POLY_128 = 0;
 constexpr float PT_RESCALE = 8.f;       // log2 of the largest probability kept unscaled
 
 template <int HD>
@@ -100,28 +98,6 @@ __device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
     return r;
 }
-// 2^x of two values at most 2^7, on the FMA pipe: x = n + f with |f| <= 1/2 (n read off the low bits of
-// x + 1.5 * 2^23), 2^f by a polynomial of degree 4 (least largest relative error on the interval:
-// 2.6e-6, far below a probability's rounding to 16 bits), n added to its exponent. Values below -126 are
-// taken as -126: a probability that rounds to nothing. The exponential unit does four a cycle and
-// scheduler, which alone would take as long as the MMAs at head_dim 128 and twice as long at 64.
-__device__ __forceinline__ void exp2_poly(F2 x, float& r0, float& r1) {
-    float a, b;
-    f2_split(x, a, b);
-    x = f2(fmaxf(a, -126.f), fmaxf(b, -126.f));
-    const F2 magic = f2(12582912.f, 12582912.f), minus = f2(-12582912.f, -12582912.f), neg = f2(-1.f, -1.f);
-    const F2 t = f2_add(x, magic), f = f2_fma(f2_add(t, minus), neg, x);
-    F2 p = f2_fma(f2(0.009570100344717503f, 0.009570100344717503f), f, f2(0.05591786280274391f, 0.05591786280274391f));
-    p = f2_fma(p, f, f2(0.240247443318367f, 0.240247443318367f));
-    p = f2_fma(p, f, f2(0.6931217908859253f, 0.6931217908859253f));
-    p = f2_fma(p, f, f2(0.9999992847442627f, 0.9999992847442627f));
-    float t0, t1, p0, p1;
-    f2_split(t, t0, t1);
-    f2_split(p, p0, p1);
-    r0 = __int_as_float(__float_as_int(p0) + (__float_as_int(t0) << 23));
-    r1 = __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23));
-}
-
 // MMAs and commits of a converged warp, issued by its elected lane: with the warp together the
 // descriptors stay in uniform registers, where a branch for one lane moves them there for each MMA.
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
@@ -326,101 +302,131 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars->q_ready[g]);
         }
-        float mref = -INFINITY, sum = 0.f;
+        // Tiles [plain_from, plain_to) of this block's share are seen whole by every row of the row tile.
+        const int plain_to = a.key_valid ? 0 : (pos_first + 1) / PT_KT - first;
+        const int plain_from = a.window && pos_last >= a.window ? (pos_last - a.window) / PT_KT + 1 - first : 0;
+        const F2 scale2 = f2(scale, scale);
+        float mref = -INFINITY;
+        F2 acc[4] = {f2(0.f, 0.f), f2(0.f, 0.f), f2(0.f, 0.f), f2(0.f, 0.f)};       // the row's sum, in eight parts
         bool ok = true;
         for (int j = 0; j < ngg; ++j) {
+            const bool plain = j >= plain_from && j < plain_to;
             const int k0 = (first + j) * PT_KT;
             uint32_t vw[4] = {~0u, ~0u, ~0u, ~0u};
-            if (a.key_valid)
+            if (__builtin_expect(!plain, 0)) {
+                if (a.key_valid)
 #pragma unroll
-                for (int w = 0; w < 4; ++w) vw[w] = valid_word(a, seq, k0 + w * 32);
-            const bool whole = (vw[0] & vw[1] & vw[2] & vw[3]) == ~0u;
-            const bool dead_keys = k0 < lo || k0 + PT_KT > hi || !whole;
-            const bool plain = k0 + PT_KT - 1 <= pos_first && (!a.window || k0 > pos_last - a.window) && whole;
-            if (dead_keys && g == (j < ng[0] ? 0 : 1)) {
-                // values of keys that no row of the block sees: zeros instead of what stands there
-                const int i = 2 * j + 1;
-                if (!(ok = role_wait_warp(&bars->full[i % L::STAGES], (i / L::STAGES) & 1, abort, a.err))) break;
-                const int key = k0 + t;
-                const uint32_t word = t < 64 ? (t < 32 ? vw[0] : vw[1]) : (t < 96 ? vw[2] : vw[3]);
-                const bool valid = ((word >> lane) & 1) || (a.self_visible && key >= base);
-                if (key < lo || key >= hi || !valid) {
-                    uint8_t* v = ring + i % L::STAGES * L::SLOT + t * 128;
+                    for (int w = 0; w < 4; ++w) vw[w] = valid_word(a, seq, k0 + w * 32);
+                const bool dead_keys = k0 < lo || k0 + PT_KT > hi || (vw[0] & vw[1] & vw[2] & vw[3]) != ~0u;
+                if (dead_keys && g == (j < ng[0] ? 0 : 1)) {
+                    // values of keys that no row of the block sees: zeros instead of what stands there
+                    const int i = 2 * j + 1;
+                    if (!(ok = role_wait_warp(&bars->full[i % L::STAGES], (i / L::STAGES) & 1, abort, a.err))) break;
+                    const int key = k0 + t;
+                    const uint32_t word = t < 64 ? (t < 32 ? vw[0] : vw[1]) : (t < 96 ? vw[2] : vw[3]);
+                    const bool valid = ((word >> lane) & 1) || (a.self_visible && key >= base);
+                    if (key < lo || key >= hi || !valid) {
+                        uint8_t* v = ring + i % L::STAGES * L::SLOT + t * 128;
 #pragma unroll
-                    for (int h = 0; h < HD / 64; ++h)
+                        for (int h = 0; h < HD / 64; ++h)
 #pragma unroll
-                        for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(v + h * L::HALF + (((c + t) & 7) << 4)) = make_uint4(0, 0, 0, 0);
+                            for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(v + h * L::HALF + (((c + t) & 7) << 4)) = make_uint4(0, 0, 0, 0);
+                    }
+                    fence_proxy_async();
                 }
-                fence_proxy_async();
             }
             if (!(ok = role_wait_warp(&bars->s_full[g], j & 1, abort, a.err))) break;
             tc_fence_after();
-            // a quarter of the scores is loaded while the maximum of the one before is taken
-            uint32_t s[4][32];
+            // The reference of the earlier tiles serves this one too unless the maximum passes it by more
+            // than 2^8, so the first half of the probabilities is made with it while the scores come in, a
+            // quarter at a time, and made again in the rare other case.
+            uint32_t s[4][32], pk[32];
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            tmem_ld32(ts, s[0]);
+            F2 off2;
+            auto reference = [&]() {
+                const float off = mref == -INFINITY ? 0.f : -mref;
+                off2 = f2(off, off);
+            };
+            auto quarter = [&](const uint32_t (&x)[32], uint32_t* to16) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                tmem_ld_wait32(s[c]);
-                if (c < 3) tmem_ld32(ts + (c + 1) * 32, s[c + 1]);
-                if (!plain) {
+                for (int e = 0; e < 16; ++e) {
+                    const F2 y = f2_fma(f2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), scale2, off2);
+                    float e0, e1;
+                    f2_split(y, e0, e1);
+                    e0 = exp2_ftz(e0);
+                    e1 = exp2_ftz(e1);
+                    acc[e & 3] = f2_add(acc[e & 3], f2(e0, e1));
+                    to16[e] = Pair<T>::down(e0, e1);
+                }
+            };
+            auto hand_over = [&](int half) {
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars->p_ready[g][half]);
+            };
+            auto maximum = [&](const uint32_t (&x)[32]) {
+#pragma unroll
+                for (int e = 0; e < 32; e += 2)
+                    mx[(e / 2) & 3] = fmaxf(fmaxf(mx[(e / 2) & 3], __uint_as_float(x[e])), __uint_as_float(x[e + 1]));
+            };
+            tmem_ld32(ts, s[0]);
+            // (the common way is laid out in one run: a jump costs a fetch from far behind the instruction cache)
+            if (__builtin_expect(plain, 1)) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    tmem_ld_wait32(s[c]);
+                    if (c < 3) tmem_ld32(ts + (c + 1) * 32, s[c + 1]);
+                    maximum(s[c]);
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    tmem_ld_wait32(s[c]);
+                    if (c < 3) tmem_ld32(ts + (c + 1) * 32, s[c + 1]);
                     const int w0 = k0 + c * 32;
                     const uint32_t see = (vw[c] & range32(from, pos, w0)) | (a.self_visible ? range32(pos, pos, w0) : 0u);
 #pragma unroll
                     for (int e = 0; e < 32; ++e)
                         if (!((see >> e) & 1u)) s[c][e] = __float_as_uint(-INFINITY);
+                    maximum(s[c]);
                 }
-#pragma unroll
-                for (int e = 0; e < 32; e += 2)
-                    mx[(e / 2) & 3] = fmaxf(fmaxf(mx[(e / 2) & 3], __uint_as_float(s[c][e])), __uint_as_float(s[c][e + 1]));
             }
             const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
-            const bool need = mref != -INFINITY && mt > mref + PT_RESCALE;
-            float factor = 1.f;
-            if (need) { factor = exp2_ftz(mref - mt); sum *= factor; }
-            if (need || mref == -INFINITY) mref = mt;
-            if (__any_sync(0xffffffffu, need)) {
+            const bool need = mt > mref + PT_RESCALE;                  // (and where nothing was seen before)
+            if (__builtin_expect(__any_sync(0xffffffffu, need), 0)) {
+                const float factor = need ? exp2_ftz(mref - mt) : 1.f;
+                if (need) mref = mt;
+                const F2 f = f2(factor, factor), zero = f2(0.f, 0.f);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[i] = f2_fma(acc[i], f, zero);
+                if (j > 0) {
 #pragma unroll 1
-                for (int c0 = 0; c0 < HD; c0 += 32) {
-                    uint32_t o[32];
-                    tmem_ld32(to + c0, o);
-                    tmem_ld_wait();
+                    for (int c0 = 0; c0 < HD; c0 += 32) {
+                        uint32_t o[32];
+                        tmem_ld32(to + c0, o);
+                        tmem_ld_wait();
 #pragma unroll
-                    for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * factor);
-                    tmem_st32(to + c0, o);
-                }
-            }
-            const float off = mref == -INFINITY ? 0.f : mref;
-            const F2 scale2 = f2(scale, scale), off2 = f2(-off, -off);
-            F2 ps[4] = {f2(0.f, 0.f), f2(0.f, 0.f), f2(0.f, 0.f), f2(0.f, 0.f)};
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                uint32_t pk[32];
-#pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    const int c = half * 2 + e / 16, k = (e % 16) * 2;
-                    const F2 x = f2_fma(f2(__uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1])), scale2, off2);
-                    float e0, e1;
-                    if (e % PT_POLY_OF < (HD == 64 ? PT_POLY_64 : PT_POLY_128)) {
-                        exp2_poly(x, e0, e1);
-                    } else {
-                        f2_split(x, e0, e1);
-                        e0 = exp2_ftz(e0);
-                        e1 = exp2_ftz(e1);
+                        for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * factor);
+                        tmem_st32(to + c0, o);
                     }
-                    ps[e & 3] = f2_add(ps[e & 3], f2(e0, e1));
-                    pk[e] = Pair<T>::down(e0, e1);
                 }
-                tmem_st32(ts + half * 32, pk);
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bars->p_ready[g][half]);
             }
-            const F2 both = f2_add(f2_add(ps[0], ps[1]), f2_add(ps[2], ps[3]));
+            reference();
+            quarter(s[0], pk);
+            quarter(s[1], pk + 16);
+            tmem_st32(ts, pk);
+            quarter(s[2], reinterpret_cast<uint32_t*>(s[0]));
+            hand_over(0);
+            quarter(s[3], reinterpret_cast<uint32_t*>(s[0]) + 16);
+            tmem_st32(ts + 32, s[0]);
+            hand_over(1);
+        }
+        float sum;
+        {
             float s0, s1;
-            f2_split(both, s0, s1);
-            sum += s0 + s1;
+            f2_split(f2_add(f2_add(acc[0], acc[1]), f2_add(acc[2], acc[3])), s0, s1);
+            sum = s0 + s1;
         }
         if (ok && ngg > 0) ok = role_wait_warp(&bars->o_full[g], 0, abort, a.err);
         if (ok) {

@@ -95,6 +95,16 @@ TIMESTRAL_API int tsb_dequant_prologue(timestral_ctx* ctx, int32_t on);
  * H = 256). The forecast is the same bits either way; on = 0 computes every token as the
  * reference does (src/encoder.cpp:45-106 then src/predict_block.cpp:15-16 slices). */
 TIMESTRAL_API int tsb_decoder_tail(timestral_ctx* ctx, int32_t on);
+/* Decode cache (on = 1; off by default): a forecast of more than one decode block (H beyond 32
+ * patches of the 209M geometry) without covariates, of one-row series (V = 1) on the tensor-core
+ * path, keeps the keys and values of its time sublayers between the blocks in a paged cache (the
+ * operators below), so that a block after the first runs on the patches fed back since and its
+ * decoder tokens alone instead of its whole context (reference src/forecaster.cpp:19-67). The
+ * forecast stays within the f16 path's deviation but is not the same bits: the attention over the
+ * cache sums in another order. A forecast whose context slides past max_context, one of several
+ * rows per series, tsb_attention_kernels mode 1, and one whose cache would take more than half of
+ * the free device memory run as with on = 0. */
+TIMESTRAL_API int tsb_decode_cache(timestral_ctx* ctx, int32_t on);
 /* CUDA-graph replay (on by default): a forecast without covariates that fits one decode
  * block (H <= 32 patches of the 209M geometry) is captured into a CUDA graph on its second
  * call with the same sizes, flags and device buffers (tsb_forecast_device pointers, or the

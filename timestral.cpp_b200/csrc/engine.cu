@@ -11,6 +11,7 @@
 #include "engine.cuh"
 #include "gguf.hpp"
 #include "gemm_tc.cuh"
+#include "paged.cuh"
 #include "rows.cuh"
 
 #include <algorithm>
@@ -209,6 +210,81 @@ struct Engine::Impl {
     struct RowMap { int group = 0, stride = 0, offset = 0; };
     RowMap a_map, tail;
     int tail_rows = 0;
+    // Decode cache: the time sublayers' keys and values of a multi-block forecast's context patches,
+    // one paged cache per sublayer (rows of `width` pages of kCachePage patches, [page][head][slot][64]),
+    // so that a block after the first runs on the patches fed back since and its decoder tokens
+    // alone. A block's decoder tokens sit behind the context and are written over by the next block.
+    static constexpr int kCachePage = 32;
+    struct DecodeCache {
+        bool enabled = false;    // allowed
+        bool on = false;         // used by the running forecast
+        int held = 0;            // context patches in the cache
+        int width = 0;           // pages of a row
+        int sublayer = 0;        // time sublayers run so far in the current block
+        DevBuf kv, table, q_start, lengths, feat, rope, workspace;
+    } cache;
+    int time_sublayers() const {
+        int n = 0;
+        for (const auto& layer : attn)
+            for (const AttnW& a : layer) n += a.time;
+        return n;
+    }
+    // Decide for a forecast of R2 rows whose longest context is `context` patches, with blocks of at
+    // most h patches, and lay the cache out.
+    void start_cache(int R2, int context, int h) {
+        cache.on = false;
+        cache.held = 0;
+        const int width = (context + h + kCachePage - 1) / kCachePage;
+        const size_t need = size_t(time_sublayers()) * 2 * R2 * width * kCachePage * H * 64 * sizeof(__half);
+        if (need > cache.kv.bytes) {
+            size_t free_bytes = 0, total = 0;
+            check(cudaMemGetInfo(&free_bytes, &total), "cudaMemGetInfo");
+            if (need > free_bytes / 2) return;               // the blocks run their whole context again
+        }
+        cache.kv.ensure(need);
+        cache.width = width;
+        cache.table.ensure(size_t(R2) * width * 4);
+        cache.q_start.ensure(size_t(R2 + 1) * 4);
+        cache.lengths.ensure(size_t(R2) * 4);
+        cache.on = true;
+    }
+    // The time sublayer's attention over the cache: q, k, v, gate token-major [R2 * S][H][64].
+    void cached_attention(int R2, int S, const MaskMeta& mm, const __half* gate, __half* out) {
+        const size_t pool = size_t(R2) * cache.width * kCachePage * H * 64;
+        PagedCache c;
+        c.k = cache.kv.as<__half>() + size_t(2 * cache.sublayer) * pool;
+        c.v = static_cast<__half*>(c.k) + pool;
+        c.k_slot = c.v_slot = 64;
+        c.k_head = c.v_head = int64_t(kCachePage) * 64;
+        c.k_page = c.v_page = int64_t(H) * kCachePage * 64;
+        c.table = cache.table.as<int>();
+        c.table_stride = cache.width;
+        c.num_pages = R2 * cache.width;
+        while ((1 << c.page_shift) < kCachePage) ++c.page_shift;
+        c.kv_heads = H;
+        c.head_dim = 64;
+        PagedBatch b;
+        b.q_start = cache.q_start.as<int>(); b.lengths = cache.lengths.as<int>();
+        b.seqs = R2; b.max_chunk = S; b.max_length = cache.held + S; b.tokens = R2 * S;
+        auto heads = [&](const __half* p) { PagedHeads h; h.data = const_cast<__half*>(p); h.token = D; h.head = 64; return h; };
+        PagedAppend ap;
+        ap.cache = c; ap.batch = b; ap.k = heads(kb.as<__half>()); ap.v = heads(vb.as<__half>()); ap.err = err.as<int>();
+        run("append", [&] { return paged_append(ap, false, s); });
+        PagedAttention at;
+        at.cache = c; at.batch = b; at.q = heads(qb.as<__half>()); at.out = heads(out);
+        if (gate) at.gate = heads(gate);
+        at.q_heads = H; at.group = 1; at.self_visible = 1;
+        at.scale_log2 = 0.125f * 1.4426950408889634f;
+        at.key_valid = mm.key_valid; at.key_valid_stride = mm.kv_words; at.key_valid_positions = mm.N;
+        at.err = err.as<int>();
+        const PagedPlan plan = paged_plan(at);
+        if (plan.splits > 1) {
+            cache.workspace.ensure(size_t(plan.splits) * plan.split_bytes);
+            paged_workspace(&at, cache.workspace.p, cache.workspace.bytes);
+        }
+        run("attention", [&] { return paged_attention(at, false, s); });
+        ++cache.sublayer;
+    }
     // raw covariate request inputs and assembly scratch
     DevBuf cov_ctx, cov_umask, cov_past, cov_known, cov_cpast, cov_cknown, cov_first, cov_scratch;
     // request-sized buffers kept across calls (no allocation on the forecast path once warm)
@@ -719,7 +795,11 @@ struct Engine::Impl {
         Range block_range("predict_block");
         const int W = cov ? T + h * ps : T;
         const int N = W / ps, L = T / ps;
-        const int S = cov ? 2 * N : N + h;
+        // Tokens of a row that this block runs: all of them, or behind a decode cache the patches it does not
+        // hold yet and the decoder tokens; E of them are context patches.
+        const bool cached = cache.on && !cov;
+        const int E = cached ? N - cache.held : N;
+        const int S = cov ? 2 * N : E + h;
         geo.rows = R2; geo.S = S; geo.L = L; geo.blocks = first ? 1 : geo.blocks + 1;
         const int P_all = cov ? N : h;
         const int kvw = (N + 31) / 32;
@@ -744,22 +824,45 @@ struct Engine::Impl {
                 return known_rows(rc, rows_p, mask_p, role.as<int8_t>(), R2, W, (L - 1) * ps, feat.as<float>(),
                                   aloc.as<float>(), ascale.as<float>(), s);
             });
+        const bool partial = E < N;
+        int* rope_all = rope_row.as<int>();
+        if (partial) {
+            cache.rope.ensure(size_t(R2) * (N + h) * 4);
+            rope_all = cache.rope.as<int>();
+        }
         run("positions", [&] {
-            return positions(rc, first_obs.as<int>(), R2, group_rows, N, S, cov, rope_row.as<int>(), gbeg.as<int>(),
+            return positions(rc, first_obs.as<int>(), R2, group_rows, N, partial ? N + h : S, cov, rope_all, gbeg.as<int>(),
                              gsize.as<int>(), err.as<int>(), s);
         });
-        // Patch projection (reference src/head.cpp:329-340) into token rows r*S + p, p < N.
+        const float* features = feat.as<float>();
+        if (partial) {
+            // the new patches' and decoder tokens' positions, and the new patches' features
+            check(cudaMemcpy2DAsync(rope_row.p, size_t(S) * 4, rope_all + (N - E), size_t(N + h) * 4, size_t(S) * 4, R2,
+                                    cudaMemcpyDeviceToDevice, s), "copy");
+            cache.feat.ensure(size_t(R2) * E * 2 * ps * 4);
+            check(cudaMemcpy2DAsync(cache.feat.p, size_t(E) * 2 * ps * 4, features + size_t(N - E) * 2 * ps, size_t(N) * 2 * ps * 4,
+                                    size_t(E) * 2 * ps * 4, R2, cudaMemcpyDeviceToDevice, s), "copy");
+            features = cache.feat.as<float>();
+        }
+        if (cached) {
+            cache.sublayer = 0;
+            run("append", [&] {
+                return paged_uniform_batch(R2, S, cache.held + S, cache.width, cache.q_start.as<int>(), cache.lengths.as<int>(),
+                                           cache.table.as<int>(), s);
+            });
+        }
+        // Patch projection (reference src/head.cpp:329-340) into token rows r*S + p, p < E.
         x.ensure(size_t(M) * D * 4);
-        const int64_t PR = int64_t(R2) * N;
+        const int64_t PR = int64_t(R2) * E;
         ph.ensure(size_t(PR) * 4 * D * (tc ? 2 : 4));
         {
             SimtGemm g;
-            g.A = feat.as<float>(); g.lda = 2 * ps; g.W = p_hid; g.M = int(PR); g.N = 4 * D; g.K = 2 * ps;
+            g.A = features; g.lda = 2 * ps; g.W = p_hid; g.M = int(PR); g.N = 4 * D; g.K = 2 * ps;
             g.order = ORDER_CHAIN; g.epi = tc ? SEPI_SILU_F16 : SEPI_SILU_F32; g.bias = pb_hid; g.out = ph.p; g.ldo = 4 * D;
             SimtGemm r;
-            r.A = feat.as<float>(); r.lda = 2 * ps; r.W = p_res; r.M = int(PR); r.N = D; r.K = 2 * ps;
+            r.A = features; r.lda = 2 * ps; r.W = p_res; r.M = int(PR); r.N = D; r.K = 2 * ps;
             r.order = ORDER_CHAIN; r.epi = SEPI_F32; r.bias = pb_res; r.out = x.p; r.ldo = D;
-            r.row_group = N; r.row_stride = S;
+            r.row_group = E; r.row_stride = S;
             if (patch_tc) {
                 // Tensor cores on the f16 hi/lo split of the features; rows with a feature
                 // outside the split's range are recomputed by the CUDA-core kernels.
@@ -769,7 +872,7 @@ struct Engine::Impl {
                 check(cudaMemsetAsync(pflag.p, 0, sizeof(int) + size_t(PR), s), "memset");
                 int8_t* row_flags = pflag.as<int8_t>() + sizeof(int);
                 run("patch_split", [&] {
-                    return split_f16(feat.as<float>(), PR, 2 * ps, feat16.as<__half>(), pflag.as<int>(), row_flags, s);
+                    return split_f16(features, PR, 2 * ps, feat16.as<__half>(), pflag.as<int>(), row_flags, s);
                 });
                 GemmArgs h;
                 h.A = feat16.as<__half>(); h.lda = K3; h.B = p_hid_split; h.ldb = K3; h.M = int(PR); h.N = 4 * D; h.K = K3;
@@ -777,7 +880,7 @@ struct Engine::Impl {
                 gemm(EPI_SILU, h);
                 GemmArgs o;
                 o.A = feat16.as<__half>(); o.lda = K3; o.B = p_res_split; o.ldb = K3; o.M = int(PR); o.N = D; o.K = K3;
-                o.epi.out = x.p; o.epi.ldo = D; o.epi.bias = pb_res; o.epi.row_group = N; o.epi.row_stride = S;
+                o.epi.out = x.p; o.epi.ldo = D; o.epi.bias = pb_res; o.epi.row_group = E; o.epi.row_stride = S;
                 gemm(EPI_F32, o);
                 // Only the rows with such a feature are rewritten, so every row's result is
                 // the same whatever else is in the batch.
@@ -791,17 +894,17 @@ struct Engine::Impl {
             GemmArgs a;
             a.A = ph.as<__half>(); a.lda = 4 * D; a.B = p_out; a.ldb = 4 * D; a.M = int(PR); a.N = D; a.K = 4 * D;
             a.epi.out = x.p; a.epi.ldo = D; a.epi.bias = pb_out; a.epi.resid = x.as<float>();
-            a.epi.row_group = N; a.epi.row_stride = S;
+            a.epi.row_group = E; a.epi.row_stride = S;
             block_b(a, p_out_blk);
             gemm(EPI_RESID, a);
         } else {
             SimtGemm g;
             g.A = ph.as<float>(); g.lda = 4 * D; g.W = f_pout; g.M = int(PR); g.N = D; g.K = 4 * D;
             g.order = ORDER_PANEL192; g.round_a_f16 = round_a; g.epi = SEPI_RESID; g.bias = pb_out; g.out = x.p; g.ldo = D;
-            g.row_group = N; g.row_stride = S;
+            g.row_group = E; g.row_stride = S;
             sgemm(g);
         }
-        run("fill", [&] { return fill_query(query, x.as<float>(), R2, S, N, D, s); });
+        run("fill", [&] { return fill_query(query, x.as<float>(), R2, S, E, D, s); });
 
         MaskMeta mm;
         mm.key_valid = kv.as<uint32_t>(); mm.kv_words = kvw; mm.N = N; mm.L = L; mm.S = S; mm.cov = cov;
@@ -825,7 +928,7 @@ struct Engine::Impl {
         bool tail_ok = tc && tail_enabled && !cov && group_rows == 1 && h > 0 && 128 % h == 0 && !attn[last].empty() &&
                        attn[last][0].time;
         for (size_t j = 1; tail_ok && j < attn[last].size(); ++j) tail_ok = !attn[last][j].time;
-        tail = RowMap{h, S, N};
+        tail = RowMap{h, S, E};
         tail_rows = R2 * h;
         for (size_t li = 0; li < attn.size(); ++li) {
             Range layer_range("layer %d", int(li));
@@ -885,7 +988,7 @@ struct Engine::Impl {
         Range head_range("out_norm + quantile head + refine");
         const int DR = R2 * P_all;
         dec.ensure(size_t(DR) * D * eb);
-        run("rms", [&] { return rms_norm(x.as<float>(), out_norm, DR, D, mv.eps, dec.p, tc, P_all, S, N, s); });
+        run("rms", [&] { return rms_norm(x.as<float>(), out_norm, DR, D, mv.eps, dec.p, tc, P_all, S, E, s); });
         const int NQ = ps * Q;
         hh.ensure(size_t(DR) * 4 * D * eb);
         hraw.ensure(size_t(DR) * NQ * 4);
@@ -920,6 +1023,7 @@ struct Engine::Impl {
             c.round_a_f16 = round_a; c.epi = SEPI_RESID; c.out = hraw.p; c.ldo = NQ;
             sgemm(c);
         }
+        if (cached) cache.held = N;
         const int steps = h * ps;
         qout.ensure(size_t(R2) * steps * Q * 4);
         run("head", [&] {
@@ -977,12 +1081,15 @@ struct Engine::Impl {
             consume(g.epi);
             g.epi.qkvg[0] = qb.as<__half>(); g.epi.qkvg[1] = kb.as<__half>(); g.epi.qkvg[2] = vb.as<__half>();
             g.epi.qkvg[3] = gb.as<__half>();
-            g.epi.S = S; g.epi.H = H; g.epi.D = D; g.epi.rope = a.time;
+            const bool cached = cache.on && a.time;      // token-major q, k, v and gate: rows of one token
+            g.epi.S = cached ? 1 : S; g.epi.H = H; g.epi.D = D; g.epi.rope = a.time;
             g.epi.cos_tab = cos_tab; g.epi.sin_tab = sin_tab; g.epi.rope_row = rope_row.as<int>(); g.epi.rope_half = rope_half;
             g.epi.rope_dup = rope_dup;
             gemm(EPI_QKVG, g);
             const __half* gate = a.gate ? gb.as<__half>() : nullptr;
-            if (attn_simt && a.time && S <= kSimtMaxKeys) {
+            if (cached) {
+                cached_attention(R2, S, mm, gate, att16);
+            } else if (attn_simt && a.time && S <= kSimtMaxKeys) {
                 run("attention", [&] { return attention_time_simt<__half>(qb.as<__half>(), kb.as<__half>(), vb.as<__half>(), gate, att16, R2, H, hd, mm, s); });
             } else if (attn_simt && !a.time) {
                 run("attention_variate", [&] { return attention_variate_simt<__half>(qb.as<__half>(), kb.as<__half>(), vb.as<__half>(), gate, att16, R2, H, hd, mm, s); });
@@ -1202,6 +1309,13 @@ void Engine::targets_body(const float* d_ctx, const uint8_t* d_umask, int B, int
     int Tc = len, done = 0;
     const bool single = patches <= shot;
     if (!single) im.decoded.ensure(size_t(R2) * H * Q * 4);
+    // The decode cache serves blocks whose context only grows (no slide), of one-row series: then a patch's
+    // features, key bit and position stay what they were. (A row without any observation gets its first
+    // one, and with it other positions, from the fed back medians; its older patches stay unseen.)
+    const int longest = len + (patches - 1) / shot * shot * ps;
+    im.cache.on = false;
+    if (im.cache.enabled && !single && im.tc && im.hd == 64 && V == 1 && !im.attn_simt && longest <= cap)
+        im.start_cache(R2, longest / ps, shot);
     (void)T;
     while (done < patches) {
         const int block = std::min(shot, patches - done), n = block * ps, offset = done * ps;
@@ -1263,6 +1377,10 @@ void Engine::decoder_tail(bool on) {
     impl_->tail_enabled = on;
     impl_->drop_graph();
     impl_->have_last = false;
+}
+
+void Engine::decode_cache(bool on) {
+    impl_->cache.enabled = on;
 }
 
 void Engine::set_observer(const BlockObserver* observer) {
@@ -1458,6 +1576,7 @@ void Engine::forecast_covariates(const CovRequest& q, bool symmetric, bool clip,
 void Engine::decode_rows(int B, int V, int H, int R, int T, int Hh, bool symmetric, bool clip, bool cov,
                          bool has_future, int group_rows, int cap, float* h_out, float* h_decoded) {
     Impl& im = *impl_;
+    im.cache.on = false;
     const ModelView& mv = im.mv;
     const int ps = im.ps, Q = im.Q;
     const int R2 = symmetric ? 2 * R : R;

@@ -148,6 +148,10 @@ public:
     // whose norm gain is folded into them keep the f16 copy unless the gain is 1. Returns
     // false when the model has no block-quantised weights (and `on` was asked).
     bool dequant_prologue(bool on);
+    // Decode cache (off by default): a multi-block forecast without covariates of one-row series keeps
+    // the time sublayers' keys and values between its blocks (tensor-core path), so that a block after
+    // the first runs on the patches fed back since and its decoder tokens alone.
+    void decode_cache(bool on);
     // Observe every decode block of the following forecasts (nullptr: none). While an
     // observer is set, forecasts are not captured into or replayed from CUDA graphs.
     void set_observer(const BlockObserver* observer);

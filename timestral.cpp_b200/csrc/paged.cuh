@@ -136,6 +136,12 @@ struct PagedPlan {
 };
 PagedPlan paged_plan(const PagedAttention& a);
 
+// Give a call the workspace: as many splits as it holds, its partial results laid out in it.
+void paged_workspace(PagedAttention* a, void* workspace, size_t bytes);
+
+// A batch of `seqs` sequences of `length` positions, the last `chunk` of them new, whose pages lie one
+// behind the other in the pool, `width` to a sequence.
+cudaError_t paged_uniform_batch(int seqs, int chunk, int length, int width, int* q_start, int* lengths, int* table, cudaStream_t stream);
 // bf16: values of type bf16, else f16.
 cudaError_t norm_rope(const NormRope& a, bool bf16, cudaStream_t stream);
 cudaError_t paged_append(const PagedAppend& a, bool bf16, cudaStream_t stream);

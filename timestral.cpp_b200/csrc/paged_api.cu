@@ -274,14 +274,6 @@ extern "C" TIMESTRAL_API int tsb_paged_attention(const tsb_paged_attention_args*
         (a->workspace_bytes && !on_device(r, a->workspace, "workspace", dev)) || !error_word(r, a->error, dev))
         return r.report();
     tsb::PagedAttention p = attention_of(*a);
-    const tsb::PagedPlan plan = tsb::paged_plan(p);
-    const size_t held = a->workspace && plan.split_bytes ? a->workspace_bytes / plan.split_bytes : 0;
-    p.splits = held < 2 ? 1 : int(held < size_t(plan.splits) ? held : size_t(plan.splits));
-    if (p.splits > 1) {
-        // weighted values, then their (maximum, sum) pairs
-        const size_t rows = size_t(p.splits) * size_t(plan.items - plan.whole) * plan.tile_rows;
-        p.part_o = static_cast<float*>(a->workspace);
-        p.part_ml = reinterpret_cast<float2*>(p.part_o + rows * a->cache->head_dim);
-    }
+    if (a->workspace_bytes) tsb::paged_workspace(&p, a->workspace, a->workspace_bytes);
     return launched(r, tsb::paged_attention(p, a->cache->type == TSB_TYPE_BF16, static_cast<cudaStream_t>(stream)));
 }

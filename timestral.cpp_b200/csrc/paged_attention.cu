@@ -592,7 +592,7 @@ cudaError_t dispatch_rows(const PagedAttention& a, const PagedGrid& grid, const 
     const bool join = plan.join;
     switch (plan.tile_rows) {
         case 8: return join ? launch_rows<T, HD, 1, 1, true, false>(a, grid, stream) : launch_rows<T, HD, 1, 1, false, false>(a, grid, stream);
-        case 16: return join ? launch_rows<T, HD, 1, 2, true, false>(a, grid, stream) : launch_rows<T, HD, 1, 2, false, false>(a, grid, stream);
+        case 16: return join ? launch_rows<T, HD, 1, 2, true, false>(a, grid, stream) : launch_rows<T, HD, 2, 1, false, false>(a, grid, stream);
         case 32: return join ? launch_rows<T, HD, 2, 2, true, false>(a, grid, stream) : launch_rows<T, HD, 2, 2, false, false>(a, grid, stream);
         default: return launch_rows<T, HD, 4, 2, false, false>(a, grid, stream);     // one team
     }
@@ -674,6 +674,15 @@ PagedPlan paged_plan(const PagedAttention& a) {
     }
     p.split_bytes = size_t(p.items - p.whole) * p.tile_rows * (size_t(a.cache.head_dim) * 4 + 8);
     return p;
+}
+
+void paged_workspace(PagedAttention* a, void* workspace, size_t bytes) {
+    const PagedPlan p = paged_plan(*a);
+    const size_t held = workspace && p.split_bytes ? bytes / p.split_bytes : 0;
+    a->splits = held < 2 ? 1 : int(std::min<size_t>(held, size_t(p.splits)));
+    // weighted values, then their (maximum, sum) pairs
+    a->part_o = static_cast<float*>(workspace);
+    a->part_ml = reinterpret_cast<float2*>(a->part_o + size_t(a->splits) * size_t(p.items - p.whole) * p.tile_rows * a->cache.head_dim);
 }
 
 cudaError_t paged_attention(const PagedAttention& a, bool bf16, cudaStream_t stream) {

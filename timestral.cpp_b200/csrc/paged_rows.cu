@@ -179,6 +179,13 @@ __global__ void __launch_bounds__(kThreads, U == 1 ? 4 : 3)
     }
 }
 
+__global__ void uniform_batch_kernel(int seqs, int chunk, int length, int width, int* q_start, int* lengths, int* table) {
+    const int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
+    if (i <= seqs) q_start[i] = int(i) * chunk;
+    if (i < seqs) lengths[i] = length;
+    if (i < int64_t(seqs) * width) table[i] = int(i);
+}
+
 template <class T, int PT, int U>
 cudaError_t launch_norm_rope(const NormRope& a, cudaStream_t stream) {
     constexpr int PER = kThreads / PT;
@@ -227,6 +234,13 @@ cudaError_t launch_append(const PagedAppend& a, cudaStream_t stream) {
 }
 
 }  // namespace
+
+cudaError_t paged_uniform_batch(int seqs, int chunk, int length, int width, int* q_start, int* lengths, int* table, cudaStream_t stream) {
+    const int64_t n = std::max(int64_t(seqs) + 1, int64_t(seqs) * width);
+    if (n > INT32_MAX || int64_t(seqs) * chunk > INT32_MAX) return cudaErrorInvalidValue;
+    uniform_batch_kernel<<<unsigned((n + kThreads - 1) / kThreads), kThreads, 0, stream>>>(seqs, chunk, length, width, q_start, lengths, table);
+    return cudaGetLastError();
+}
 
 cudaError_t norm_rope(const NormRope& a, bool bf16, cudaStream_t stream) {
     return bf16 ? dispatch_norm_rope<__nv_bfloat16>(a, stream) : dispatch_norm_rope<__half>(a, stream);

@@ -516,6 +516,17 @@ TIMESTRAL_API int tsb_decoder_tail(timestral_ctx* c, int32_t on) {
     return TSB_OK;
 }
 
+TIMESTRAL_API int tsb_decode_cache(timestral_ctx* c, int32_t on) {
+    if (!c) return TSB_ERR_ARG;
+    try {
+        for (size_t k = 0; k < c->gpus(); ++k) c->gpu(k).engine().decode_cache(on != 0);
+    } catch (...) {
+        caught(c);
+        return TSB_ERR_CUDA;
+    }
+    return TSB_OK;
+}
+
 TIMESTRAL_API int tsb_graph_replay(timestral_ctx* c, int32_t on) {
     if (!c) return TSB_ERR_ARG;
     try {

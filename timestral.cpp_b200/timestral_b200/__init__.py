@@ -122,6 +122,7 @@ SIGNATURES = {
     "tsb_graph_replay": (C.c_int, [C.c_void_p, C.c_int32]),
     "tsb_fused_norm": (C.c_int, [C.c_void_p, C.c_int32]),
     "tsb_attention_kernels": (C.c_int, [C.c_void_p, C.c_int32]),
+    "tsb_decode_cache": (C.c_int, [C.c_void_p, C.c_int32]),
     "tsb_decoder_tail": (C.c_int, [C.c_void_p, C.c_int32]),
     "tsb_dequant_prologue": (C.c_int, [C.c_void_p, C.c_int32]),
     "tsb_test_scale_rows": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_double] + [C.c_int32] * 6
@@ -277,6 +278,12 @@ class Model:
         """Last layer's per-token work on the decoder tokens alone (default on; same bits)."""
         if lib().tsb_decoder_tail(self.h, int(on)) != 0:
             raise RuntimeError("tsb_decoder_tail failed")
+
+    def decode_cache(self, on: bool):
+        """Keep the time sublayers' keys and values between the blocks of a multi-block forecast
+        (default off)."""
+        if lib().tsb_decode_cache(self.h, int(on)) != 0:
+            raise RuntimeError("tsb_decode_cache failed")
 
     def graph_replay(self, on: bool):
         """CUDA-graph replay of repeated single-block forecasts (on by default)."""

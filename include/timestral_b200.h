@@ -283,9 +283,9 @@ TIMESTRAL_API int tsb_paged_append(const tsb_paged_append_args* args, void* stre
  * self_visible adding j = p whatever its bit. A token that sees nothing gives zeros. What stands in
  * the cache at positions that no token of the sequence sees (NaN too) does not reach the results.
  * gate (as q) may be NULL; out may be q itself. scale 0 means 1 / sqrt(head_dim).
- * The keys of few rows are split between blocks, as far as `workspace` holds their partial
- * results; tsb_paged_attention_workspace gives the bytes that the call can use at most (NULL and 0
- * are allowed). A workspace serves one call at a time: calls that may overlap on the GPU (other
+ * The keys of few rows are split between blocks, beyond a few splits as far as `workspace` holds
+ * their partial results; tsb_paged_attention_workspace gives the bytes that the call can use at
+ * most (NULL and 0 are allowed). A workspace serves one call at a time: calls that may overlap on the GPU (other
  * streams, two graphs) need one each. Results do not depend on what it held. */
 typedef struct tsb_paged_attention_args {
     const tsb_paged_cache* cache;
@@ -302,7 +302,7 @@ typedef struct tsb_paged_attention_args {
 } tsb_paged_attention_args;
 TIMESTRAL_API int tsb_paged_attention(const tsb_paged_attention_args* args, void* stream);
 /* Bytes of workspace that lets a call with these arguments split as it would like to (0: it
- * does not split). Only cache, batch (bounds), tokens, q_heads and window are read. */
+ * needs none). Only cache, batch (bounds), tokens, q_heads and window are read. */
 TIMESTRAL_API size_t tsb_paged_attention_workspace(const tsb_paged_attention_args* args);
 
 /* ---- kernel-level test entries (device pointers) ---------------------------------- */

@@ -307,13 +307,15 @@ def test_attention_strides_scale_and_output_in_place(new, lengths, order):
     assert torch.equal(b.q, other)
 
 
-@pytest.mark.parametrize("new, lengths", [([1], [3000]), ([4, 1], [900, 2000]), ([150], [2000])])
-def test_attention_splits_as_far_as_the_workspace_goes(new, lengths):
+@pytest.mark.parametrize("new, lengths, wanted", [([1], [3000], True), ([4, 1], [900, 2000], False), ([4, 1], [900, 9000], True),
+                                                  ([150], [2000], True)])
+def test_attention_splits_as_far_as_the_workspace_goes(new, lengths, wanted):
+    """A few splits join without a workspace (wanted False); more want one, and take what there is."""
     b = ref.Batch(new, lengths, 4, 2, 128, 64, torch.float16)
     want, tol = ref.attention(b)
     full = tb.paged_attention_workspace(*handles(b), b.tokens, b.qh)
-    assert full > 0
-    for size in (0, 4, full // 4, full // 2, full - 4, "full"):
+    assert (full > 0) == wanted
+    for size in (0, 4, full // 4, full // 2, max(full - 4, 0), "full"):
         a = attend(b, workspace=size)
         ref.within(a, want, tol)
         assert torch.equal(a, attend(b, workspace=size))          # the same bits every time

@@ -278,10 +278,8 @@ struct Engine::Impl {
         at.key_valid = mm.key_valid; at.key_valid_stride = mm.kv_words; at.key_valid_positions = mm.N;
         at.err = err.as<int>();
         const PagedPlan plan = paged_plan(at);
-        if (plan.splits > 1) {
-            cache.workspace.ensure(size_t(plan.splits) * plan.split_bytes);
-            paged_workspace(&at, cache.workspace.p, cache.workspace.bytes);
-        }
+        if (plan.splits > std::max(plan.cluster, 1)) cache.workspace.ensure(size_t(plan.splits) * plan.split_bytes);
+        paged_workspace(&at, cache.workspace.p, cache.workspace.bytes);
         run("attention", [&] { return paged_attention(at, false, s); });
         ++cache.sublayer;
     }

@@ -103,6 +103,7 @@ struct PagedGrid {
     FastDiv splits, heads, seqs, group;
     uint32_t items = 0, whole = 0, units = 0, row_tiles = 0;
     uint32_t one_keys = 0;              // rows, a tile for all keys: the tile's keys
+    uint32_t cluster = 0;               // rows: the splits of an item are a cluster
 };
 struct PagedItem {
     int row_tile, kvh, seq;
@@ -132,11 +133,12 @@ struct PagedPlan {
     int tile_rows = 0;
     int64_t row_tiles = 0, items = 0, whole = 0;
     int splits = 1;
+    int cluster = 0;                    // splits that need no workspace
     size_t split_bytes = 0;             // workspace bytes of one split
 };
 PagedPlan paged_plan(const PagedAttention& a);
 
-// Give a call the workspace: as many splits as it holds, its partial results laid out in it.
+// Give a call its workspace (or none): as many splits as it holds, its partial results laid out in it.
 void paged_workspace(PagedAttention* a, void* workspace, size_t bytes);
 
 // A batch of `seqs` sequences of `length` positions, the last `chunk` of them new, whose pages lie one

@@ -260,7 +260,7 @@ extern "C" TIMESTRAL_API size_t tsb_paged_attention_workspace(const tsb_paged_at
     if (!attention_shape(r, a, false)) { r.report(); return 0; }
     if (!a->tokens || !a->batch->seqs || !a->batch->max_chunk) return 0;
     const tsb::PagedPlan p = tsb::paged_plan(attention_of(*a));
-    return p.splits > 1 ? size_t(p.splits) * p.split_bytes : 0;
+    return p.splits > 1 && p.splits > p.cluster ? size_t(p.splits) * p.split_bytes : 0;
 }
 
 extern "C" TIMESTRAL_API int tsb_paged_attention(const tsb_paged_attention_args* a, void* stream) {
@@ -274,6 +274,6 @@ extern "C" TIMESTRAL_API int tsb_paged_attention(const tsb_paged_attention_args*
         (a->workspace_bytes && !on_device(r, a->workspace, "workspace", dev)) || !error_word(r, a->error, dev))
         return r.report();
     tsb::PagedAttention p = attention_of(*a);
-    if (a->workspace_bytes) tsb::paged_workspace(&p, a->workspace, a->workspace_bytes);
+    tsb::paged_workspace(&p, a->workspace, a->workspace_bytes);
     return launched(r, tsb::paged_attention(p, a->cache->type == TSB_TYPE_BF16, static_cast<cudaStream_t>(stream)));
 }

@@ -47,7 +47,7 @@ struct RowsLayout {
     static constexpr int RING = STAGES * 2 * TILE;
     static constexpr int SMEM = 1024 + TEAMS * RING + TEAMS * STAGES * 8;
     static int smem(int keys) { return ONE ? 1024 + TEAMS * (2 * HD / 64 * keys * 128 + 8) : SMEM; }
-    static_assert(SMEM >= 4 * 16 * HD * 4 + 4 * 16 * 8, "the joined rows reuse the rings");
+    static_assert(ONE || SMEM >= 1024 + (4 * 16 + 16 * RG) * (HD * 4 + 8), "the joined rows reuse the rings");
 };
 
 template <class T>
@@ -92,6 +92,18 @@ struct RowTile {
     int lo, hi;                  // keys that any row of the tile may see
     int start;                   // first token row
 };
+
+// 16 bytes (8) of another block of the cluster, at this block's shared address.
+__device__ __forceinline__ float4 peer_load4(const void* mine, uint32_t rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(mapa_shared(smem_u32(mine), rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ float2 peer_load2(const void* mine, uint32_t rank) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(mapa_shared(smem_u32(mine), rank)) : "memory");
+    return v;
+}
 
 // Eight finished values (columns 8 c ..) of a row: normalised, gated, rounded, stored.
 template <class T>
@@ -466,6 +478,8 @@ __global__ void __launch_bounds__(PR_THREADS, HD == 128 ? 1 : NR == 1 ? 5 : RG =
         }
     __syncthreads();
     constexpr int CH = HD / 8;
+    float* share_o = reinterpret_cast<float*>(smem) + 4 * WR * HD + 8 * WR;        // behind the warps' rows and sums
+    float2* share_ml = reinterpret_cast<float2*>(share_o + MT * HD);
     for (int i = threadIdx.x; i < t.rows * CH; i += PR_THREADS) {
         const int r = i / CH, c = i % CH, g = r / WR, rr = r % WR;
         float m = -INFINITY;
@@ -482,6 +496,13 @@ __global__ void __launch_bounds__(PR_THREADS, HD == 128 ? 1 : NR == 1 ? 5 : RG =
 #pragma unroll
             for (int e = 0; e < 8; ++e) y[e] = fmaf(src[e], f, y[e]);
         }
+        if (splits > 1 && grid.cluster) {
+            float4* dst = reinterpret_cast<float4*>(share_o + r * HD + c * 8);
+            dst[0] = make_float4(y[0], y[1], y[2], y[3]);
+            dst[1] = make_float4(y[4], y[5], y[6], y[7]);
+            if (c == 0) share_ml[r] = make_float2(m, l);
+            continue;
+        }
         if (splits > 1) {
             const int64_t at = part + r;
             if (c == 0) a.part_ml[at] = make_float2(m, l);
@@ -496,6 +517,30 @@ __global__ void __launch_bounds__(PR_THREADS, HD == 128 ? 1 : NR == 1 ? 5 : RG =
         int head;
         row_of(r, &token, &head);
         store_row<T>(a, token, head, c, y, m == -INFINITY ? 0.f : 1.0f / l);
+    }
+    if (splits > 1 && grid.cluster) {
+        // The splits of an item are one cluster: each block finishes its share of the rows from all of them.
+        cluster_sync();
+        for (int i = int(split) * PR_THREADS + threadIdx.x; i < t.rows * CH; i += splits * PR_THREADS) {
+            const int r = i / CH, c = i % CH;
+            float m = -INFINITY;
+            for (int k = 0; k < splits; ++k) m = fmaxf(m, peer_load2(share_ml + r, k).x);
+            float y[8] = {}, l = 0.f;
+            for (int k = 0; k < splits; ++k) {
+                const float2 ml = peer_load2(share_ml + r, k);
+                const float f = ml.x == -INFINITY ? 0.f : exp2_ftz(ml.x - m);
+                const float4 u = peer_load4(share_o + r * HD + c * 8, k), w = peer_load4(share_o + r * HD + c * 8 + 4, k);
+                const float p[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+                l = fmaf(ml.y, f, l);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = fmaf(p[e], f, y[e]);
+            }
+            int64_t token;
+            int head;
+            row_of(r, &token, &head);
+            store_row<T>(a, token, head, c, y, m == -INFINITY ? 0.f : 1.0f / l);
+        }
+        cluster_sync();                             // no block leaves while another reads its shared memory
     }
 }
 
@@ -578,8 +623,18 @@ cudaError_t launch_rows(const PagedAttention& a, const PagedGrid& grid, cudaStre
     PageMaps maps;
     if (!page_maps(&maps, a.cache, std::is_same<T, __nv_bfloat16>::value, L::BOX)) return cudaErrorInvalidValue;
     const unsigned blocks = JOIN ? grid.units : (grid.units + L::TEAMS - 1) / L::TEAMS;
-    paged_rows_kernel<T, HD, RG, NR, JOIN, ONE><<<blocks, PR_THREADS, L::smem(int(grid.one_keys)), stream>>>(maps, a, grid);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3(PR_THREADS);
+    cfg.dynamicSmemBytes = L::smem(int(grid.one_keys));
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = unsigned(a.splits);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = JOIN && grid.cluster ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, paged_rows_kernel<T, HD, RG, NR, JOIN, ONE>, maps, a, grid);
 }
 template <class T, int HD>
 cudaError_t dispatch_rows(const PagedAttention& a, const PagedGrid& grid, const PagedPlan& plan, cudaStream_t stream) {
@@ -619,7 +674,7 @@ template <class T, int HD>
 cudaError_t dispatch(const PagedAttention& a, const PagedPlan& plan, const PagedGrid& grid, cudaStream_t stream) {
     const cudaError_t e = plan.tiles ? paged_attention_tiles(a, grid, std::is_same<T, __nv_bfloat16>::value, stream)
                                      : dispatch_rows<T, HD>(a, grid, plan, stream);
-    if (e != cudaSuccess || a.splits == 1) return e;
+    if (e != cudaSuccess || a.splits == 1 || grid.cluster) return e;
     return a.splits > 4 ? launch_combine<T, HD, 8>(a, grid, plan.tile_rows, stream) : launch_combine<T, HD, 2>(a, grid, plan.tile_rows, stream);
 }
 
@@ -670,7 +725,10 @@ PagedPlan paged_plan(const PagedAttention& a) {
     } else {
         p.one = !a.window && a.batch.max_length <= 96;
         p.join = rows <= 32 && keys > 256;
+        // Up to 8 splits of a problem are a cluster whose blocks join in shared memory; more go through the
+        // workspace and a second kernel.
         p.splits = int(std::max<int64_t>(1, std::min<int64_t>({p.items >= sms ? (4 * sms + p.items - 1) / p.items : sms / p.items, (keys + 255) / 256, 256})));
+        if (p.join && p.splits > 1) p.cluster = std::min(p.splits, 8);
     }
     p.split_bytes = size_t(p.items - p.whole) * p.tile_rows * (size_t(a.cache.head_dim) * 4 + 8);
     return p;
@@ -679,7 +737,11 @@ PagedPlan paged_plan(const PagedAttention& a) {
 void paged_workspace(PagedAttention* a, void* workspace, size_t bytes) {
     const PagedPlan p = paged_plan(*a);
     const size_t held = workspace && p.split_bytes ? bytes / p.split_bytes : 0;
+    a->part_o = nullptr;
+    a->part_ml = nullptr;
     a->splits = held < 2 ? 1 : int(std::min<size_t>(held, size_t(p.splits)));
+    if (p.cluster >= a->splits) a->splits = p.cluster;     // a cluster's blocks join their splits without it
+    if (a->splits == 1 || p.cluster == a->splits) return;
     // weighted values, then their (maximum, sum) pairs
     a->part_o = static_cast<float*>(workspace);
     a->part_ml = reinterpret_cast<float2*>(a->part_o + size_t(a->splits) * size_t(p.items - p.whole) * p.tile_rows * a->cache.head_dim);
@@ -698,6 +760,7 @@ cudaError_t paged_attention(const PagedAttention& a, bool bf16, cudaStream_t str
     g.whole = uint32_t(whole);
     g.units = uint32_t(units);
     g.row_tiles = uint32_t(p.row_tiles);
+    g.cluster = a.splits > 1 && !a.part_o;
     g.one_keys = uint32_t(std::max(16, (a.batch.max_length + 15) / 16 * 16));
     if (a.cache.head_dim == 64) return bf16 ? dispatch<__nv_bfloat16, 64>(a, p, g, stream) : dispatch<__half, 64>(a, p, g, stream);
     return bf16 ? dispatch<__nv_bfloat16, 128>(a, p, g, stream) : dispatch<__half, 128>(a, p, g, stream);

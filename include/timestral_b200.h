@@ -281,7 +281,8 @@ TIMESTRAL_API int tsb_paged_append(const tsb_paged_append_args* args, void* stre
  * with window > 0 those with j > p - window, and with key_valid those whose bit is set (bit j % 32
  * of word j / 32 of the sequence's row; positions from key_valid_positions on count as set),
  * self_visible adding j = p whatever its bit. A token that sees nothing gives zeros. What stands in
- * the cache at positions that no token of the sequence sees (NaN too) does not reach the results.
+ * the cache at positions that no new token sees (NaN too) does not reach the results; a value (v)
+ * that is not finite at a position that some new token sees may reach all of that sequence's.
  * gate (as q) may be NULL; out may be q itself. scale 0 means 1 / sqrt(head_dim).
  * The keys of few rows are split between blocks, beyond a few splits as far as `workspace` holds
  * their partial results; tsb_paged_attention_workspace gives the bytes that the call can use at

@@ -397,6 +397,29 @@ def test_attention_large_scores_and_repeated_maxima():
         ref.within(attend(b), want, tol)
 
 
+@pytest.mark.parametrize("new, lengths", [([1, 1], [40, 3000]), ([4, 1], [4, 900]), ([150, 1], [2000, 30]), ([1, 1], [5, 96])])
+def test_attention_hands_on_what_is_not_a_number(new, lengths):
+    """A query or a visible key that is NaN gives NaN in its rows, however the keys are split, and nowhere
+    else; an infinite score does too (inf - inf)."""
+    for bad in (NAN, math.inf):
+        b = ref.Batch(new, lengths, 4, 2, 128, 16, torch.float16)
+        want, tol = ref.attention(b)
+        b.q[0, 1] = NAN                                            # one head of the first token
+        if math.isinf(bad):
+            b.q[0, 1] = 1.0
+            b.k_pool[b.table[0, 0], 0, 0] = bad                    # seen by every token of sequence 0, heads 0 and 1
+        hit = torch.zeros(b.tokens, 4, dtype=torch.bool, device="cuda")
+        if math.isinf(bad):
+            hit[:new[0], :2] = True
+        else:
+            hit[0, 1] = True
+        for workspace in ("full", None):
+            out = attend(b, workspace=workspace)
+            if not math.isinf(bad):
+                assert torch.isnan(out[hit]).all()
+            ref.within(out[~hit], want[~hit], tol[~hit])
+
+
 def test_calls_refuse_other_memory():
     b = ref.Batch([1, 4], [20, 9], 4, 2, 64, 16, torch.float16)
     cache, batch = handles(b)

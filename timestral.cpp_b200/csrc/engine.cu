@@ -92,6 +92,13 @@ struct DevBuf {
               "cudaMalloc workspace");
         bytes = std::max<size_t>(n, 256);
     }
+    void release() {
+        if (!p) return;
+        g_workspace_generation.fetch_add(1);
+        cudaFree(p);
+        p = nullptr;
+        bytes = 0;
+    }
     template <class T> T* as() const { return static_cast<T*>(p); }
 };
 
@@ -1378,7 +1385,13 @@ void Engine::decoder_tail(bool on) {
 }
 
 void Engine::decode_cache(bool on) {
-    impl_->cache.enabled = on;
+    Impl& im = *impl_;
+    if (!on && im.cache.kv.p) {
+        check(cudaSetDevice(device_), "cudaSetDevice");
+        check(cudaStreamSynchronize(stream_), "sync");
+        im.cache.kv.release();
+    }
+    im.cache.enabled = on;
 }
 
 void Engine::set_observer(const BlockObserver* observer) {

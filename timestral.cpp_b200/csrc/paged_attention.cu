@@ -93,6 +93,10 @@ struct RowTile {
     int start;                   // first token row
 };
 
+// Of a partial result: no key was seen. (Scores that are all NaN leave the maximum where it was, too,
+// and a sum that is NaN.)
+__device__ __forceinline__ bool saw_nothing(float maximum, float sum) { return maximum == -INFINITY && sum == 0.f; }
+
 // 16 bytes (8) of another block of the cluster, at this block's shared address.
 __device__ __forceinline__ float4 peer_load4(const void* mine, uint32_t rank) {
     float4 v;
@@ -418,7 +422,7 @@ __global__ void __launch_bounds__(PR_THREADS, HD == 128 ? 1 : NR == 1 ? 5 : RG =
                     if (pos[n][e] < 0) continue;
                     const int64_t at = part + rg * WR + n * 8 + (lane & 3) * 2 + e;
                     if (lane < 4) a.part_ml[at] = make_float2(mx[n][e], sum[n][e]);
-                    if (mx[n][e] == -INFINITY) continue;
+                    if (saw_nothing(mx[n][e], sum[n][e])) continue;
 #pragma unroll
                     for (int d = 0; d < MD; ++d) {
                         a.part_o[at * HD + d * 16 + (lane >> 2)] = o[d][n][e];
@@ -506,7 +510,7 @@ __global__ void __launch_bounds__(PR_THREADS, HD == 128 ? 1 : NR == 1 ? 5 : RG =
         if (splits > 1) {
             const int64_t at = part + r;
             if (c == 0) a.part_ml[at] = make_float2(m, l);
-            if (m != -INFINITY) {
+            if (!saw_nothing(m, l)) {
                 float4* dst = reinterpret_cast<float4*>(a.part_o + at * HD + c * 8);
                 dst[0] = make_float4(y[0], y[1], y[2], y[3]);
                 dst[1] = make_float4(y[4], y[5], y[6], y[7]);
@@ -568,7 +572,7 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttention
 #pragma unroll 4
         for (int s = g; s < a.splits; s += G) {
             const float2 ml = a.part_ml[s * step + at];
-            if (ml.x == -INFINITY) continue;          // saw nothing: no partial row was written
+            if (saw_nothing(ml.x, ml.y)) continue;    // no partial row was written
             const float4* src = reinterpret_cast<const float4*>(a.part_o + (s * step + at) * HD + c * 8);
             const float4 u = src[0], w = src[1];
             const float top = fmaxf(top_m, ml.x), f = exp2_ftz(ml.x - top), old = exp2_ftz(top_m - top);
@@ -593,7 +597,7 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttention
 #pragma unroll
     for (int k = 0; k < G; ++k) {
         const float2 ml = sml[slot + k];
-        if (ml.x == -INFINITY) continue;
+        if (saw_nothing(ml.x, ml.y)) continue;
         const float f = exp2_ftz(ml.x - top);
         l = fmaf(ml.y, f, l);
 #pragma unroll

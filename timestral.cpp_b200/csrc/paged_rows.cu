@@ -107,8 +107,9 @@ __global__ void __launch_bounds__(kThreads, U == 1 ? 4 : 3) norm_rope_kernel(con
 }
 
 // A block: new tokens of one sequence, U cached heads a thread, their keys and values.
-template <class T, int PT, int U>
-__global__ void __launch_bounds__(kThreads, U == 1 ? 4 : 3)
+// PLAIN: neither norm nor rotation, so fewer registers and more blocks an SM.
+template <class T, int PT, int U, bool PLAIN>
+__global__ void __launch_bounds__(kThreads, PLAIN ? 8 : U == 1 ? 4 : 3)
     paged_append_kernel(const PagedAppend a, const FastDiv blocks, const FastDiv units, float inv_dim) {
     uint32_t in_seq, first;
     const int seq = int(blocks.divmod(blockIdx.x, &in_seq));
@@ -139,7 +140,7 @@ __global__ void __launch_bounds__(kThreads, U == 1 ? 4 : 3)
     }
     bool writes = live;
     if (live && (page < 0 || page >= c.num_pages)) { record_error(a.err, kDevBadPage); writes = false; }
-    if (a.k_weight || a.rot.cos) {
+    if constexpr (!PLAIN) {
         float cs[8] = {}, sn[8] = {}, w0[8] = {}, w1[8] = {};
         bool turned = false;
         if (live && a.rot.cos) {
@@ -218,19 +219,22 @@ cudaError_t dispatch_norm_rope(const NormRope& a, cudaStream_t stream) {
     return launch_norm_rope<T, 16>(a, stream);
 }
 
-template <class T, int PT, int U>
+template <class T, int PT, int U, bool PLAIN>
 cudaError_t launch_append(const PagedAppend& a, cudaStream_t stream) {
     const int64_t units = (a.cache.kv_heads + U - 1) / U;
     const int64_t per_seq = (int64_t(a.batch.max_chunk) * units + kThreads / PT - 1) / (kThreads / PT);
     if (per_seq * a.batch.seqs > INT32_MAX || per_seq * (kThreads / PT) > INT32_MAX) return cudaErrorInvalidValue;
-    paged_append_kernel<T, PT, U><<<unsigned(per_seq * a.batch.seqs), kThreads, 0, stream>>>(a, FastDiv(uint32_t(per_seq)), FastDiv(uint32_t(units)),
+    paged_append_kernel<T, PT, U, PLAIN><<<unsigned(per_seq * a.batch.seqs), kThreads, 0, stream>>>(a, FastDiv(uint32_t(per_seq)), FastDiv(uint32_t(units)),
                                                                                                1.0f / float(a.cache.head_dim));
     return cudaGetLastError();
 }
 template <class T, int PT>
 cudaError_t launch_append(const PagedAppend& a, cudaStream_t stream) {
-    return a.cache.kv_heads >= 2 && int64_t(a.batch.max_chunk) * a.batch.seqs * a.cache.kv_heads * PT >= 148 * 2048
-               ? launch_append<T, PT, 2>(a, stream) : launch_append<T, PT, 1>(a, stream);
+    // a plain copy: a head a thread and all the blocks an SM holds (2048 rows of 16 tokens: 38.3 us, with two
+    // heads a thread and five blocks 39.6); else two heads where there is work for all SMs
+    if (!a.k_weight && !a.rot.cos) return launch_append<T, PT, 1, true>(a, stream);
+    const bool two = a.cache.kv_heads >= 2 && int64_t(a.batch.max_chunk) * a.batch.seqs * a.cache.kv_heads * PT >= 148 * 2048;
+    return two ? launch_append<T, PT, 2, false>(a, stream) : launch_append<T, PT, 1, false>(a, stream);
 }
 
 }  // namespace

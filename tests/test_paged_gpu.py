@@ -307,8 +307,8 @@ def test_attention_strides_scale_and_output_in_place(new, lengths, order):
     assert torch.equal(b.q, other)
 
 
-@pytest.mark.parametrize("new, lengths, wanted", [([1], [3000], True), ([4, 1], [900, 2000], False), ([4, 1], [900, 9000], True),
-                                                  ([150], [2000], True)])
+@pytest.mark.parametrize("new, lengths, wanted", [([1], [3000], False), ([4, 1], [900, 2000], False), ([4, 1], [900, 9000], True),
+                                                  ([150], [2000], True), ([1], [30000], True)])
 def test_attention_splits_as_far_as_the_workspace_goes(new, lengths, wanted):
     """A few splits join without a workspace (wanted False); more want one, and take what there is."""
     b = ref.Batch(new, lengths, 4, 2, 128, 64, torch.float16)

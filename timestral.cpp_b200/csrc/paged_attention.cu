@@ -8,6 +8,7 @@
 #include "paged.cuh"
 
 #include <algorithm>
+#include <atomic>
 #include <climits>
 
 namespace tsb {
@@ -682,6 +683,39 @@ cudaError_t dispatch(const PagedAttention& a, const PagedPlan& plan, const Paged
     return a.splits > 4 ? launch_combine<T, HD, 8>(a, grid, plan.tile_rows, stream) : launch_combine<T, HD, 2>(a, grid, plan.tile_rows, stream);
 }
 
+// Blocks of joined teams that the device runs at once in clusters of n: with one block an SM a cluster of
+// 8 leaves 28 of the 148 SMs idle, a cluster of 2 none. Asked once for each device and layout.
+template <int HD, int RG, int NR>
+int cluster_blocks(int n) {
+    static std::atomic<int> counts[64][8];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) dev = 0;
+    int blocks = counts[dev][n - 1].load(std::memory_order_relaxed);
+    if (blocks) return blocks;
+    using L = RowsLayout<HD, RG, false>;
+    const auto kernel = paged_rows_kernel<__half, HD, RG, NR, true, false>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(n));
+    cfg.blockDim = dim3(PR_THREADS);
+    cfg.dynamicSmemBytes = L::SMEM;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = unsigned(n);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int clusters = 0;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess || clusters < 1) {
+        cudaGetLastError();                               // no device: the plan is still one that runs
+        return device_sm_count() * (8 * 64 / HD * RG / 4) * 7 / 8;
+    }
+    blocks = clusters * n;
+    counts[dev][n - 1].store(blocks, std::memory_order_relaxed);
+    return blocks;
+}
+
 }  // namespace
 
 // A tensor map over one of the pools, its axes in order of stride (an axis of one entry has none of
@@ -706,34 +740,102 @@ bool page_maps(PageMaps* m, const PagedCache& c, bool bf16, int box_slots) {
            page_map(&m->v, c.v, bf16, c, c.v_page, c.v_head, c.v_slot, box_slots);
 }
 
+// Which way to run a call: an estimate in microseconds of each, and the least is taken. It goes by sizes
+// alone (the bounds that the host knows; the lengths stand on the device). Rounds of units (a problem's
+// keys or a share of them), each with a start and its keys, where a unit goes at the rate of its own
+// teams' loads or at its part of what an SM loads, whichever is slower. The constants below were fitted
+// to the best choice over 7,534 calls (1 to 256 rows, 97 to 16,484 keys, 1 to 512 sequences, 2 to 16
+// cached heads, even and uneven lengths), each timed in every way open to it: on average the chosen way
+// took 1.02 times the best one's time, 1.14 at the 95th percentile, 1.42 at worst. Fixed bounds on rows
+// and keys (teams joined above 256 keys, tiles above 64 rows) took 1.14, 1.66 and 4.4.
+// Both sides, us: one row over 500 keys of 64, 24,576 problems: a team each 520, teams joined 604, and
+// over 800 keys, 96 problems: 33 and 16; 64 rows over 4,016 keys of 128, 512 problems: rows 303, tiles 242,
+// and over 128 keys of 64, 12,288 problems: rows 213, tiles 555; 16 problems over 11,000 keys of 128, clusters
+// of 6 and of 8 (one too many for a round): 31 and 45.
+struct RowsChoice {
+    double us = 0;
+    bool join = false;
+    int splits = 1;
+};
+static RowsChoice rows_choice(int tile_rows, int head_dim, int64_t items, int64_t keys, int64_t sms) {
+    const int at = tile_rows == 8 ? 0 : tile_rows == 16 ? 1 : tile_rows == 32 ? 2 : 3;
+    const bool wide = head_dim == 128;
+    // us a key: of what an SM loads, a problem's part at each size of rows; and of what a team loads
+    constexpr double kShared[2][4] = {{.0046, .0046, .0052, .0110}, {.0061, .0074, .0075, .0113}}, kTeam = .0245;
+    const double shared = kShared[wide][at];
+    const int teams = (wide ? 4 : 8) / (at == 3 ? 2 : 1), joined = at == 3 ? 1 : at == 2 ? 2 : 4;      // of an SM, of a block
+    RowsChoice best;
+    auto consider = [&](bool join, int64_t splits) {
+        const int block = join ? joined : 1;
+        const bool cluster = join && splits > 1 && splits <= 8;
+        int64_t slots = sms * teams / block;
+        if (cluster) {
+            const int n = int(splits);
+            slots = wide ? at == 0 ? cluster_blocks<128, 1, 1>(n) : at == 1 ? cluster_blocks<128, 1, 2>(n) : cluster_blocks<128, 2, 2>(n)
+                         : at == 0 ? cluster_blocks<64, 1, 1>(n) : at == 1 ? cluster_blocks<64, 1, 2>(n) : cluster_blocks<64, 2, 2>(n);
+        }
+        const int64_t units = items * splits, rounds = units / slots, rest = units % slots;
+        const double start = (join ? 3.7 : 2.9) + (cluster ? 1.1 + .13 * double(splits) : 0);
+        auto round = [&](int64_t at_once) {
+            return at_once ? start + double(keys) / double(splits) * std::max(kTeam / block, double(at_once) / double(sms) * shared) : 0;
+        };
+        // uneven lengths and starts leave about a third of a round behind the last
+        double us = double(rounds) * round(slots) + round(rest) + .35 * round(rounds ? slots : rest);
+        // a second kernel, and the partial rows through the workspace
+        if (splits > 1 && !cluster) us += 2.7 + .1 * double(splits) + 4.2e-7 * double(units * tile_rows) * (head_dim * 4 + 8);
+        if (best.us == 0 || us < best.us) best = {us, join, int(splits)};
+    };
+    consider(false, 1);
+    const bool join = joined > 1;
+    for (int64_t n = join ? 1 : 2; n <= 8 && (n == 1 || keys >= 32 * n); ++n) consider(join, n);
+    for (int64_t n = 1; n <= 3; ++n) {
+        const int64_t splits = std::min<int64_t>(sms * teams / joined * n / items, 256);
+        if (splits > 8 && keys >= 64 * splits) consider(join, splits);
+    }
+    return best;
+}
+
 PagedPlan paged_plan(const PagedAttention& a) {
     PagedPlan p;
-    const int64_t rows = int64_t(a.batch.max_chunk) * a.group;
-    p.tiles = rows > 64;
-    p.tile_rows = p.tiles ? kPagedTileRows : rows_of_team(a);
-    p.row_tiles = (rows + p.tile_rows - 1) / p.tile_rows;
-    p.items = p.row_tiles * a.cache.kv_heads * a.batch.seqs;
+    const int64_t rows = int64_t(a.batch.max_chunk) * a.group, problems = int64_t(a.cache.kv_heads) * a.batch.seqs;
     const int64_t sms = device_sm_count();
     const int64_t keys = a.window ? std::min<int64_t>(a.batch.max_length, int64_t(a.window) + a.batch.max_chunk) : a.batch.max_length;
-    if (p.tiles) {
-        // As many items as fill the SMs once or more stay whole; the rest are split so that they take the
-        // least time together: rounds of blocks times a block's key tiles, of which its start and end cost
-        // about three more (and the join about four).
-        p.whole = p.items / sms * sms;
-        const int64_t rest = p.items - p.whole, tiles = (keys + 127) / 128;
-        int64_t best = INT64_MAX;
+    // tiles: as many items as fill the SMs once or more stay whole; the rest are split so that they take
+    // the least time together
+    int64_t tiles_cost = 0, tiles_whole = 0;
+    int tiles_splits = 1;
+    {
+        const int64_t items = (rows + kPagedTileRows - 1) / kPagedTileRows * problems, tiles = (keys + 127) / 128;
+        tiles_whole = items / sms * sms;
+        const int64_t rest = items - tiles_whole;
+        int64_t best = rest ? INT64_MAX : 0;
         for (int s = 1; rest && s <= 32 && (s == 1 || 2 * s <= tiles); ++s) {
             const int64_t cost = (rest * s + sms - 1) / sms * ((tiles + s - 1) / s + 3) + (s > 1 ? 4 : 0);
-            if (cost < best) { best = cost; p.splits = s; }
+            if (cost < best) { best = cost; tiles_splits = s; }
         }
+        tiles_cost = items / sms * (tiles + 3) + best;
+    }
+    p.tile_rows = rows_of_team(a);
+    p.row_tiles = (rows + p.tile_rows - 1) / p.tile_rows;
+    // 96 rows over 96 keys, 6,144 problems: one tile of keys 166 us, tcgen05 285
+    p.one = !a.window && a.batch.max_length <= 96 && rows <= kPagedTileRows;
+    RowsChoice choice;
+    if (!p.one && rows <= kPagedTileRows)
+        choice = rows_choice(p.tile_rows, a.cache.head_dim, std::max<int64_t>(p.row_tiles * problems, 1), std::max<int64_t>(keys, 1), sms);
+    p.tiles = !p.one && rows > 8 && (rows > kPagedTileRows || choice.us > 4.4 + 1.69 * double(tiles_cost));
+    if (p.tiles) {
+        p.tile_rows = kPagedTileRows;
+        p.row_tiles = (rows + kPagedTileRows - 1) / kPagedTileRows;
+        p.whole = tiles_whole;
+        p.splits = tiles_splits;
     } else {
-        p.one = !a.window && a.batch.max_length <= 96;
-        p.join = rows <= 32 && keys > 256;
+        p.join = choice.join;
+        p.splits = choice.splits;
         // Up to 8 splits of a problem are a cluster whose blocks join in shared memory; more go through the
         // workspace and a second kernel.
-        p.splits = int(std::max<int64_t>(1, std::min<int64_t>({p.items >= sms ? (4 * sms + p.items - 1) / p.items : sms / p.items, (keys + 255) / 256, 256})));
         if (p.join && p.splits > 1) p.cluster = std::min(p.splits, 8);
     }
+    p.items = p.row_tiles * problems;
     p.split_bytes = size_t(p.items - p.whole) * p.tile_rows * (size_t(a.cache.head_dim) * 4 + 8);
     return p;
 }

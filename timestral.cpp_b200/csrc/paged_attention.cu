@@ -800,14 +800,19 @@ PagedPlan paged_plan(const PagedAttention& a) {
     const int64_t rows = int64_t(a.batch.max_chunk) * a.group, problems = int64_t(a.cache.kv_heads) * a.batch.seqs;
     const int64_t sms = device_sm_count();
     const int64_t keys = a.window ? std::min<int64_t>(a.batch.max_length, int64_t(a.window) + a.batch.max_chunk) : a.batch.max_length;
+    // Row tiles that hold rows: where the new tokens are uneven, fewer than max_chunk allows (the rest of
+    // the grid ends at once). 7 prompts of 1 to 300 tokens, window 1,000, planned as if all of 300: 41 us, so: 37.
+    auto held = [&](int64_t row_tiles, int tile_rows) {
+        return std::max<int64_t>(std::min(row_tiles * a.batch.seqs, int64_t(a.batch.tokens) * a.group / tile_rows + a.batch.seqs), 1) * a.cache.kv_heads;
+    };
     // tiles: as many items as fill the SMs once or more stay whole; the rest are split so that they take
     // the least time together
     int64_t tiles_cost = 0, tiles_whole = 0;
     int tiles_splits = 1;
     {
-        const int64_t items = (rows + kPagedTileRows - 1) / kPagedTileRows * problems, tiles = (keys + 127) / 128;
-        tiles_whole = items / sms * sms;
-        const int64_t rest = items - tiles_whole;
+        const int64_t row_tiles = (rows + kPagedTileRows - 1) / kPagedTileRows, tiles = (keys + 127) / 128;
+        const int64_t items = held(row_tiles, kPagedTileRows), rest = items % sms;
+        tiles_whole = row_tiles * problems * (items - rest) / items;
         int64_t best = rest ? INT64_MAX : 0;
         for (int s = 1; rest && s <= 32 && (s == 1 || 2 * s <= tiles); ++s) {
             const int64_t cost = (rest * s + sms - 1) / sms * ((tiles + s - 1) / s + 3) + (s > 1 ? 4 : 0);
@@ -821,7 +826,7 @@ PagedPlan paged_plan(const PagedAttention& a) {
     p.one = !a.window && a.batch.max_length <= 96 && rows <= kPagedTileRows;
     RowsChoice choice;
     if (!p.one && rows <= kPagedTileRows)
-        choice = rows_choice(p.tile_rows, a.cache.head_dim, std::max<int64_t>(p.row_tiles * problems, 1), std::max<int64_t>(keys, 1), sms);
+        choice = rows_choice(p.tile_rows, a.cache.head_dim, held(p.row_tiles, p.tile_rows), std::max<int64_t>(keys, 1), sms);
     p.tiles = !p.one && rows > 8 && (rows > kPagedTileRows || choice.us > 4.4 + 1.69 * double(tiles_cost));
     if (p.tiles) {
         p.tile_rows = kPagedTileRows;

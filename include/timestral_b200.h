@@ -283,7 +283,8 @@ TIMESTRAL_API int tsb_paged_append(const tsb_paged_append_args* args, void* stre
  * self_visible adding j = p whatever its bit. A token that sees nothing gives zeros. What stands in
  * the cache at positions that no new token sees (NaN too) does not reach the results; a value (v)
  * that is not finite at a position that some new token sees may reach all of that sequence's.
- * gate (as q) may be NULL; out may be q itself. scale 0 means 1 / sqrt(head_dim).
+ * gate (as q) may be NULL; out may be q itself (same strides), and otherwise overlaps nothing that the
+ * call reads. scale 0 means 1 / sqrt(head_dim).
  * The keys of few rows are split between blocks, beyond a few splits as far as `workspace` holds
  * their partial results; tsb_paged_attention_workspace gives the bytes that the call can use at
  * most (NULL and 0 are allowed). A workspace serves one call at a time: calls that may overlap on the GPU (other

@@ -275,6 +275,35 @@ def test_attention_key_valid(hd, self_visible, share, new, lengths, qh, kvh):
 
 
 @pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("window", [0, 40])
+@pytest.mark.parametrize("new, lengths, qh, kvh", [([50], [90], 4, 1), ([90, 3, 40], [96, 70, 40], 4, 2), ([64], [300], 4, 1),
+                                                   ([100, 0, 31], [577, 5, 31], 2, 2), ([33, 2], [97, 1000], 14, 2), ([8] * 40, [120] * 40, 16, 2)])
+def test_attention_several_row_tiles_over_few_keys(hd, window, new, lengths, qh, kvh):
+    """65 to 256 rows of a problem: more than one tile of rows, each with keys of its own."""
+    b = ref.Batch(new, lengths, qh, kvh, hd, 16, torch.float16, seed=window, extra_rows=3)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    bits = torch.rand(len(new), -(-max(lengths) // 32) * 32, generator=g, device="cuda") < 0.7
+    for kw in ({}, {"bits": bits, "self_visible": True, "gate": b.gate}):
+        want, tol = ref.attention(b, window=window, **kw)
+        for workspace in ("full", None):
+            out = attend(b, window=window, workspace=workspace, **kw)
+            ref.within(out[:b.tokens], want, tol)
+            assert (out[b.tokens:] == 7).all()
+
+
+@pytest.mark.parametrize("seqs", [1, 2, 3, 5, 9, 14, 20, 37, 75, 150])
+@pytest.mark.parametrize("hd, qh, kvh", [(64, 2, 1), (128, 12, 1), (128, 8, 2), (64, 20, 1)])
+def test_attention_any_number_of_problems(seqs, hd, qh, kvh):
+    """From many splits of few problems over clusters of every size to one team a problem."""
+    lengths = [700 - 3 * (i % 50) for i in range(seqs)]
+    b = ref.Batch([1] * seqs, lengths, qh, kvh, hd, 32, torch.bfloat16, seed=seqs)
+    want, tol = ref.attention(b)
+    for workspace in ("full", None):
+        ref.within(attend(b, workspace=workspace), want, tol)
+    assert torch.equal(attend(b), attend(b))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("new, lengths", [([1, 1], [77, 300]), ([5, 30], [5, 131]), ([129, 70], [129, 400])])
 def test_attention_unused_slots_hold_anything(hd, new, lengths):
     """NaN in every slot that no sequence owns, and pages that end inside a tile."""

@@ -112,6 +112,16 @@ def test_norm_rope_refuses():
     refused(lambda: tb.norm_rope(q, q[:1].expand(3, 4, 64), cos=cos, sin=cos, positions=pos), "overlap")
 
 
+def test_outputs_in_place_keep_the_layout():
+    """The input's address with other strides: a block would write what another has not read yet."""
+    a = arrays()
+    cache, batch = handles(a)
+    q = torch.zeros(4, 4, 64, dtype=torch.float16)
+    refused(lambda: tb.paged_attention(cache, batch, q, q.transpose(0, 1)), "other strides")
+    refused(lambda: tb.norm_rope(q, q.transpose(0, 1)), "q_out is its input")
+    refused(lambda: tb.norm_rope(q, q, q, q.transpose(0, 1)), "k_out is its input")
+
+
 def test_c_entries_refuse_null():
     L = tb.lib()
     assert L.tsb_norm_rope(None, None) == tb.TSB_ERR_ARG

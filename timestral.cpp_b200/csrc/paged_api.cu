@@ -71,6 +71,11 @@ bool output_shape(Refusal& r, const tsb_heads& h, const char* name, int tokens, 
                        (h.token_stride >= head_dim && h.head_stride >= h.token_stride * (tokens - 1) + head_dim) || (heads == 1 && h.token_stride >= head_dim);
     return heads_shape(r, h, name, heads, head_dim) && r.need(apart, "%s has tokens that overlap", name);
 }
+// An output in its input's place has its layout: a block would write what another has not read yet.
+bool in_place_shape(Refusal& r, const tsb_heads& in, const tsb_heads& out, const char* name, int tokens, int heads) {
+    return r.need(in.data != out.data || ((tokens <= 1 || in.token_stride == out.token_stride) && (heads <= 1 || in.head_stride == out.head_stride)),
+                  "%s is its input with other strides", name);
+}
 
 bool rotation_shape(Refusal& r, const tsb_rotation& t, int head_dim, bool positions_needed) {
     if (!t.cos && !t.sin) return true;
@@ -175,6 +180,7 @@ bool attention_shape(Refusal& r, const tsb_paged_attention_args* a, bool pointer
         return false;
     return !pointers ||
            (heads_shape(r, a->q, "q", a->q_heads, c.head_dim) && output_shape(r, a->out, "out", a->tokens, a->q_heads, c.head_dim) &&
+            in_place_shape(r, a->q, a->out, "out", a->tokens, a->q_heads) &&
             (!a->gate.data || heads_shape(r, a->gate, "gate", a->q_heads, c.head_dim)) &&
             r.need(std::isfinite(a->scale), "scale is not finite") &&
             r.need(!a->key_valid || (a->key_valid_positions >= 0 && a->key_valid_stride >= (int64_t(a->key_valid_positions) + 31) / 32),
@@ -213,6 +219,7 @@ extern "C" TIMESTRAL_API int tsb_norm_rope(const tsb_norm_rope_args* a, void* st
         {a->q, a->q_out, a->q_weight, a->q_heads, "q", "q_out", "q_weight"}, {a->k, a->k_out, a->k_weight, a->k_heads, "k", "k_out", "k_weight"}};
     for (const auto& s : side)
         if (s.heads && (!heads_shape(r, s.in, s.name, s.heads, a->head_dim) || !output_shape(r, s.out, s.out_name, a->tokens, s.heads, a->head_dim) ||
+                        !in_place_shape(r, s.in, s.out, s.out_name, a->tokens, s.heads) ||
                         !aligned(r, s.w, s.w_name, 16)))
             return r.report();
     if (!a->tokens || (!a->q_heads && !a->k_heads)) return TSB_OK;

@@ -812,7 +812,8 @@ PagedPlan paged_plan(const PagedAttention& a) {
     {
         const int64_t row_tiles = (rows + kPagedTileRows - 1) / kPagedTileRows, tiles = (keys + 127) / 128;
         const int64_t items = held(row_tiles, kPagedTileRows), rest = items % sms;
-        tiles_whole = row_tiles * problems * (items - rest) / items;
+        const int64_t all = row_tiles * problems;             // rest of them, or as many more as end at once
+        tiles_whole = all - rest * all / items;
         int64_t best = rest ? INT64_MAX : 0;
         for (int s = 1; rest && s <= 32 && (s == 1 || 2 * s <= tiles); ++s) {
             const int64_t cost = (rest * s + sms - 1) / sms * ((tiles + s - 1) / s + 3) + (s > 1 ? 4 : 0);

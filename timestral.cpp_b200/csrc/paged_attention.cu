@@ -686,11 +686,8 @@ cudaError_t dispatch(const PagedAttention& a, const PagedPlan& plan, const Paged
 // Blocks of joined teams that the device runs at once in clusters of n: with one block an SM a cluster of
 // 8 leaves 28 of the 148 SMs idle, a cluster of 2 none. Asked once for each device and layout.
 template <int HD, int RG, int NR>
-int cluster_blocks(int n) {
+int cluster_blocks(int n, int dev, int sms) {
     static std::atomic<int> counts[64][8];
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev < 0 || dev >= 64) dev = 0;
     int blocks = counts[dev][n - 1].load(std::memory_order_relaxed);
     if (blocks) return blocks;
     using L = RowsLayout<HD, RG, false>;
@@ -709,7 +706,7 @@ int cluster_blocks(int n) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM) != cudaSuccess ||
         cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess || clusters < 1) {
         cudaGetLastError();                               // no device: the plan is still one that runs
-        return device_sm_count() * (8 * 64 / HD * RG / 4) * 7 / 8;
+        return sms * (8 * 64 / HD * RG / 4) * 7 / 8;
     }
     blocks = clusters * n;
     counts[dev][n - 1].store(blocks, std::memory_order_relaxed);
@@ -744,10 +741,10 @@ bool page_maps(PageMaps* m, const PagedCache& c, bool bf16, int box_slots) {
 // alone (the bounds that the host knows; the lengths stand on the device). Rounds of units (a problem's
 // keys or a share of them), each with a start and its keys, where a unit goes at the rate of its own
 // teams' loads or at its part of what an SM loads, whichever is slower. The constants below were fitted
-// to the best choice over 7,534 calls (1 to 256 rows, 97 to 16,484 keys, 1 to 512 sequences, 2 to 16
+// to the best choice over 9,983 calls (1 to 256 rows, 97 to 198,000 keys, 1 to 512 sequences, 2 to 16
 // cached heads, even and uneven lengths), each timed in every way open to it: on average the chosen way
-// took 1.02 times the best one's time, 1.14 at the 95th percentile, 1.42 at worst. Fixed bounds on rows
-// and keys (teams joined above 256 keys, tiles above 64 rows) took 1.14, 1.66 and 4.4.
+// took 1.02 times the best one's time, 1.13 at the 95th percentile, 1.42 at worst. Fixed bounds on rows
+// and keys (teams joined above 256 keys, tiles above 64 rows) took 1.16, 1.75 and 5.6.
 // Both sides, us: one row over 500 keys of 64, 24,576 problems: a team each 520, teams joined 604, and
 // over 800 keys, 96 problems: 33 and 16; 64 rows over 4,016 keys of 128, 512 problems: rows 303, tiles 242,
 // and over 128 keys of 64, 12,288 problems: rows 213, tiles 555; 16 problems over 11,000 keys of 128, clusters
@@ -757,13 +754,16 @@ struct RowsChoice {
     bool join = false;
     int splits = 1;
 };
-static RowsChoice rows_choice(int tile_rows, int head_dim, int64_t items, int64_t keys, int64_t sms) {
+static RowsChoice rows_choice(int tile_rows, int head_dim, int64_t items, int64_t keys, bool one_seq, int64_t sms) {
     const int at = tile_rows == 8 ? 0 : tile_rows == 16 ? 1 : tile_rows == 32 ? 2 : 3;
     const bool wide = head_dim == 128;
     // us a key: of what an SM loads, a problem's part at each size of rows; and of what a team loads
     constexpr double kShared[2][4] = {{.0046, .0046, .0052, .0110}, {.0061, .0074, .0075, .0113}}, kTeam = .0245;
     const double shared = kShared[wide][at];
     const int teams = (wide ? 4 : 8) / (at == 3 ? 2 : 1), joined = at == 3 ? 1 : at == 2 ? 2 : 4;      // of an SM, of a block
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) dev = 0;
     RowsChoice best;
     auto consider = [&](bool join, int64_t splits) {
         const int block = join ? joined : 1;
@@ -771,16 +771,17 @@ static RowsChoice rows_choice(int tile_rows, int head_dim, int64_t items, int64_
         int64_t slots = sms * teams / block;
         if (cluster) {
             const int n = int(splits);
-            slots = wide ? at == 0 ? cluster_blocks<128, 1, 1>(n) : at == 1 ? cluster_blocks<128, 1, 2>(n) : cluster_blocks<128, 2, 2>(n)
-                         : at == 0 ? cluster_blocks<64, 1, 1>(n) : at == 1 ? cluster_blocks<64, 1, 2>(n) : cluster_blocks<64, 2, 2>(n);
+            slots = (wide ? at == 0 ? cluster_blocks<128, 1, 1> : at == 1 ? cluster_blocks<128, 1, 2> : cluster_blocks<128, 2, 2>
+                          : at == 0 ? cluster_blocks<64, 1, 1> : at == 1 ? cluster_blocks<64, 1, 2> : cluster_blocks<64, 2, 2>)(n, dev, int(sms));
         }
         const int64_t units = items * splits, rounds = units / slots, rest = units % slots;
         const double start = (join ? 3.7 : 2.9) + (cluster ? 1.1 + .13 * double(splits) : 0);
         auto round = [&](int64_t at_once) {
             return at_once ? start + double(keys) / double(splits) * std::max(kTeam / block, double(at_once) / double(sms) * shared) : 0;
         };
-        // uneven lengths and starts leave about a third of a round behind the last
-        double us = double(rounds) * round(slots) + round(rest) + .35 * round(rounds ? slots : rest);
+        // uneven lengths and starts leave about a third of a round behind the last, one sequence's starts less (with
+        // a third there too 8 problems over 131,072 keys of 128 run as 55 splits each, 92 us; 18 of them: 87)
+        double us = double(rounds) * round(slots) + round(rest) + (one_seq ? .2 : .35) * round(rounds ? slots : rest);
         // a second kernel, and the partial rows through the workspace
         if (splits > 1 && !cluster) us += 2.7 + .1 * double(splits) + 4.2e-7 * double(units * tile_rows) * (head_dim * 4 + 8);
         if (best.us == 0 || us < best.us) best = {us, join, int(splits)};
@@ -809,7 +810,7 @@ PagedPlan paged_plan(const PagedAttention& a) {
     // the least time together
     int64_t tiles_cost = 0, tiles_whole = 0;
     int tiles_splits = 1;
-    {
+    if (rows > 8) {                                       // 8 rows are padded to 256: never faster
         const int64_t row_tiles = (rows + kPagedTileRows - 1) / kPagedTileRows, tiles = (keys + 127) / 128;
         const int64_t items = held(row_tiles, kPagedTileRows), rest = items % sms;
         const int64_t all = row_tiles * problems;             // rest of them, or as many more as end at once
@@ -827,7 +828,7 @@ PagedPlan paged_plan(const PagedAttention& a) {
     p.one = !a.window && a.batch.max_length <= 96 && rows <= kPagedTileRows;
     RowsChoice choice;
     if (!p.one && rows <= kPagedTileRows)
-        choice = rows_choice(p.tile_rows, a.cache.head_dim, held(p.row_tiles, p.tile_rows), std::max<int64_t>(keys, 1), sms);
+        choice = rows_choice(p.tile_rows, a.cache.head_dim, held(p.row_tiles, p.tile_rows), std::max<int64_t>(keys, 1), a.batch.seqs == 1, sms);
     p.tiles = !p.one && rows > 8 && (rows > kPagedTileRows || choice.us > 4.4 + 1.69 * double(tiles_cost));
     if (p.tiles) {
         p.tile_rows = kPagedTileRows;

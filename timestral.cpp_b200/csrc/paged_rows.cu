@@ -1,7 +1,9 @@
 // Per-head norm and rotation of queries and keys (norm_rope), and writing keys and values into
 // a paged cache with the same norm and rotation on the way (paged_append).
 //
-// Both read every value once and write it once: the memory rate bounds them. A head is held by
+// Both read every value once and write it once: the memory rate bounds them (68.5 us and 0.77
+// of the copy rate for norm and rotation of 16,384 tokens of 40 heads of 128; 24.6 us, 0.80, for 64 uneven prompts
+// of up to 512 tokens appended; 38.7 us, 0.79, for 32,768 tokens of 12 heads of 64 appended as they are). A head is held by
 // PT threads (head_dim / 16, rounded up to a power of two), each with two vectors of eight values
 // whose elements the rotation pairs (d and d + rope_dim / 2; behind rope_dim two neighbouring
 // vectors that nothing turns), so that the rotation needs no exchange and the sum of squares is
@@ -51,13 +53,29 @@ __device__ __forceinline__ void load8(const float* p, float (&f)[8]) {
     *reinterpret_cast<float4*>(f + 4) = *reinterpret_cast<const float4*>(p + 4);
 }
 
+// Sixteen bytes that this call reads (writes) once. HINT: first to leave L2, so that the copies which wait
+// there to be written back do not push out what is still to be read. Passes over the same buffers, norm and
+// rotation of 16,384 tokens of 40 heads of 128: 61.2 us, without the hint 64.5 (other buffers each time: 68.5, 68.9); a reader right behind it takes as long
+// either way (123.3 and 123.8 with it). 64 prompts of 512 tokens appended with a rotation: 20.6 and 22.9. The
+// plain copy goes without (2,048 rows of 16 tokens: 36.4, with it 37.1).
+template <bool HINT>
+__device__ __forceinline__ uint4 load16(const void* p) {
+    if constexpr (HINT) return __ldcs(static_cast<const uint4*>(p));
+    else return *static_cast<const uint4*>(p);
+}
+template <bool HINT>
+__device__ __forceinline__ void store16(void* p, const uint4& x) {
+    if constexpr (HINT) __stcs(static_cast<uint4*>(p), x);
+    else *static_cast<uint4*>(p) = x;
+}
+
 constexpr int kThreads = 256;
 
 // Blocks [0, q_blocks) norm and turn the queries, the rest the keys. A thread has U heads of one
 // token, which share its angles and weights: their table rows (f32, twice the bytes of a 16-bit head)
 // come from L1 once for U heads, and 32 U bytes of values are in flight per thread.
 template <class T, int PT, int U>
-__global__ void __launch_bounds__(kThreads, U == 1 ? 4 : 3) norm_rope_kernel(const NormRope a, int q_blocks, float inv_dim) {
+__global__ void __launch_bounds__(kThreads, 4) norm_rope_kernel(const NormRope a, int q_blocks, float inv_dim) {
     const bool is_q = int(blockIdx.x) < q_blocks;
     const NormRopeSide& s = is_q ? a.q : a.k;
     const uint32_t block = is_q ? blockIdx.x : blockIdx.x - q_blocks;
@@ -75,8 +93,8 @@ __global__ void __launch_bounds__(kThreads, U == 1 ? 4 : 3) norm_rope_kernel(con
     for (int j = 0; j < U; ++j) {
         u0[j] = u1[j] = make_uint4(0, 0, 0, 0);
         if (!here || int(first) + j >= s.heads) continue;
-        u0[j] = *reinterpret_cast<const uint4*>(in + j * s.in.head + e0);
-        u1[j] = *reinterpret_cast<const uint4*>(in + j * s.in.head + e1);
+        u0[j] = load16<true>(in + j * s.in.head + e0);
+        u1[j] = load16<true>(in + j * s.in.head + e1);
     }
     bool writes = here, turned = false;
     float c[8] = {}, sn[8] = {}, w0[8] = {}, w1[8] = {};
@@ -101,8 +119,8 @@ __global__ void __launch_bounds__(kThreads, U == 1 ? 4 : 3) norm_rope_kernel(con
         unpack8<T>(u1[j], y);
         norm_turn<PT>(x, y, s.weight != nullptr, w0, w1, a.eps, inv_dim, turned, c, sn);
         if (!writes || int(first) + j >= s.heads) continue;
-        *reinterpret_cast<uint4*>(out + j * s.out.head + e0) = pack8<T>(x);
-        *reinterpret_cast<uint4*>(out + j * s.out.head + e1) = pack8<T>(y);
+        store16<true>(out + j * s.out.head + e0, pack8<T>(x));
+        store16<true>(out + j * s.out.head + e1, pack8<T>(y));
     }
 }
 
@@ -133,10 +151,10 @@ __global__ void __launch_bounds__(kThreads, PLAIN ? 8 : U == 1 ? 4 : 3)
     for (int j = 0; j < U; ++j) {
         k0[j] = k1[j] = v0[j] = v1[j] = make_uint4(0, 0, 0, 0);
         if (!live || int(first) + j >= c.kv_heads) continue;
-        k0[j] = *reinterpret_cast<const uint4*>(k + j * a.k.head + e0);
-        k1[j] = *reinterpret_cast<const uint4*>(k + j * a.k.head + e1);
-        v0[j] = *reinterpret_cast<const uint4*>(v + j * a.v.head + e0);
-        v1[j] = *reinterpret_cast<const uint4*>(v + j * a.v.head + e1);
+        k0[j] = load16<!PLAIN>(k + j * a.k.head + e0);
+        k1[j] = load16<!PLAIN>(k + j * a.k.head + e1);
+        v0[j] = load16<!PLAIN>(v + j * a.v.head + e0);
+        v1[j] = load16<!PLAIN>(v + j * a.v.head + e1);
     }
     bool writes = live;
     if (live && (page < 0 || page >= c.num_pages)) { record_error(a.err, kDevBadPage); writes = false; }
@@ -173,10 +191,10 @@ __global__ void __launch_bounds__(kThreads, PLAIN ? 8 : U == 1 ? 4 : 3)
 #pragma unroll
     for (int j = 0; j < U; ++j) {
         if (int(first) + j >= c.kv_heads) break;
-        *reinterpret_cast<uint4*>(kd + j * c.k_head + e0) = k0[j];
-        *reinterpret_cast<uint4*>(kd + j * c.k_head + e1) = k1[j];
-        *reinterpret_cast<uint4*>(vd + j * c.v_head + e0) = v0[j];
-        *reinterpret_cast<uint4*>(vd + j * c.v_head + e1) = v1[j];
+        store16<!PLAIN>(kd + j * c.k_head + e0, k0[j]);
+        store16<!PLAIN>(kd + j * c.k_head + e1, k1[j]);
+        store16<!PLAIN>(vd + j * c.v_head + e0, v0[j]);
+        store16<!PLAIN>(vd + j * c.v_head + e1, v1[j]);
     }
 }
 
@@ -204,9 +222,10 @@ cudaError_t launch_norm_rope(const NormRope& a, cudaStream_t stream) {
 }
 template <class T, int PT>
 cudaError_t launch_norm_rope(const NormRope& a, cudaStream_t stream) {
-    // few tokens: a thread a head, for the latency; else four heads a thread where there are as many
+    // few tokens: a thread a head, for the latency; else two heads a thread where there are as many (32,768 tokens
+    // of 24 heads of 64: 37.4 us, four heads and three blocks an SM 39.4, one head 45.1)
     const int64_t heads = int64_t(a.tokens) * (a.q.heads + a.k.heads);
-    return std::max(a.q.heads, a.k.heads) >= 4 && heads * PT >= 148 * 2048 ? launch_norm_rope<T, PT, 4>(a, stream)
+    return std::max(a.q.heads, a.k.heads) >= 2 && heads * PT >= 148 * 2048 ? launch_norm_rope<T, PT, 2>(a, stream)
                                                                            : launch_norm_rope<T, PT, 1>(a, stream);
 }
 template <class T>

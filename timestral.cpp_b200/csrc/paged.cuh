@@ -212,6 +212,15 @@ struct Pair<__nv_bfloat16> {
         return *reinterpret_cast<const uint32_t*>(&h);
     }
 };
+// Probabilities are held as 2^(t - m + lift), m the row's reference maximum, which its largest score passes by
+// at most 8: rounded to f16 they reach 2^15 of its 2^16, and what its steps of 2^-24 lose lies 2^-32 below the
+// largest. Without the lift 32,768 keys of 2^-26 each behind one that stands out (w = 2^-11 of a row's weight)
+// were lost. A power of two changes no other bit, and falls out with the sum. bf16 has the range.
+template <class T>
+constexpr float kLift = 0.f;
+template <>
+inline constexpr float kLift<__half> = 7.f;
+
 // Eight 16-bit values <-> floats.
 template <class T>
 __device__ __forceinline__ void unpack8(const uint4& u, float (&f)[8]) {

@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(PR_THREADS, HD == 128 ? 1 : NR == 1 ? 5 : RG =
         for (int n = 0; n < NR; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const float ref = mx[n][e] == -INFINITY ? 0.f : mx[n][e];
+                const float ref = mx[n][e] == -INFINITY ? 0.f : mx[n][e] - kLift<T>;
 #pragma unroll
                 for (int i = 0; i < MK; ++i) {
                     sc[i][n][e] = exp2_ftz(fmaf(sc[i][n][e], scale, -ref));

@@ -12,7 +12,7 @@
 // 1.17 -> 1.36 ms for 2048 tokens of 32 heads over 34,816 keys.)
 // A commit covers every earlier MMA, so a full S_{j+1} also says that O holds tile j: the softmax
 // may rescale it. It does so only when a row's maximum passes its reference by more than 2^8
-// (probabilities then lie in (0, 256]).
+// (probabilities then lie in (0, 2^8], in f16 lifted by kLift to (0, 2^15]).
 #include "paged.cuh"
 
 #include <algorithm>
@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
             F2 off2;
             auto reference = [&]() {
-                const float off = mref == -INFINITY ? 0.f : -mref;
+                const float off = mref == -INFINITY ? 0.f : kLift<T> - mref;
                 off2 = f2(off, off);
             };
             auto quarter = [&](const uint32_t (&x)[32], uint32_t* to16) {

@@ -253,4 +253,14 @@ __device__ __forceinline__ uint32_t range32(int lo, int hi, int w0) {
     return (0xffffffffu >> (31 - hi)) & (0xffffffffu << lo);
 }
 
+// Does a new token see one of the positions [from, to), all of which lie where the rows may look? (Asked of
+// table entries that name no page: with all of a page's bits clear nobody reads it.)
+__device__ __forceinline__ bool any_valid(const PagedAttention& a, int seq, int base, int from, int to) {
+    if (!a.key_valid || (a.self_visible && to > base)) return true;
+#pragma unroll 1
+    for (int k0 = from & ~31; k0 < to; k0 += 32)
+        if (valid_word(a, seq, k0) & range32(from, to - 1, k0)) return true;
+    return false;
+}
+
 }  // namespace tsb

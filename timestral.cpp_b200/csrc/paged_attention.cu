@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(PR_THREADS, HD == 128 ? 1 : NR == 1 ? 5 : RG =
         if (rg != 0 || tile >= last || lane * box >= KT || key + box <= t.lo || key >= t.hi) return -1;
         const int page = table[key >> a.cache.page_shift];
         if (page >= 0 && page < a.cache.num_pages) return page;
-        record_error(a.err, kDevBadPage);
+        if (any_valid(a, t.seq, t.base, max(key, t.lo), min(key + box, t.hi))) record_error(a.err, kDevBadPage);
         return a.cache.num_pages;                          // outside the map: zeros
     };
     auto load_tile = [&](int tile, int stage, int page) {

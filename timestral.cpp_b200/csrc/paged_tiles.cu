@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                 if (lane * box >= PT_KT || j >= nt || key + box <= lo || key >= hi) return -1;
                 const int page = table[key >> a.cache.page_shift];
                 if (page >= 0 && page < a.cache.num_pages) return page;
-                record_error(a.err, kDevBadPage);
+                if (any_valid(a, seq, base, max(key, lo), min(key + box, hi))) record_error(a.err, kDevBadPage);
                 return a.cache.num_pages;                              // outside the map: zeros
             };
             int next = page_of(0), page = -1;

@@ -213,7 +213,7 @@ extern "C" TIMESTRAL_API int tsb_norm_rope(const tsb_norm_rope_args* a, void* st
         !r.need(a->head_dim >= 16 && a->head_dim <= 256 && a->head_dim % 16 == 0, "head_dim %d is not a multiple of 16 up to 256", a->head_dim) ||
         !r.need(a->tokens >= 0 && a->q_heads >= 0 && a->k_heads >= 0, "a size is negative") ||
         !r.need(std::isfinite(a->eps) && a->eps >= 0, "eps is negative or not finite") ||
-        !rotation_shape(r, a->rotation, a->head_dim, true))
+        !rotation_shape(r, a->rotation, a->head_dim, a->tokens > 0))       // (no token: an empty array may have no address)
         return r.report();
     const struct { const tsb_heads &in, &out; const float* w; int heads; const char *name, *out_name, *w_name; } side[2] = {
         {a->q, a->q_out, a->q_weight, a->q_heads, "q", "q_out", "q_weight"}, {a->k, a->k_out, a->k_weight, a->k_heads, "k", "k_out", "k_weight"}};

@@ -399,7 +399,10 @@ TIMESTRAL_API int tsb_test_rms(const float* x, const float* w, int32_t tokens, i
  * uses the GEMM roles' wait, 1 the attention kernels'. Takes one wait limit (about 2 s at
  * full clock), synchronizes, and returns TSB_ERR_DEVICE with the expired wait's error word
  * in *dev_error (the GEMM's stage-fill or the attention barrier code) and 1 in
- * *left_by_abort when the second role left through the flag; the context stays usable. */
+ * *left_by_abort when the second role left through the flag; the context stays usable.
+ * Kernel 2: the wait with which the paged attention kernels let their own copies land after
+ * an expired wait; *left_by_abort is 1 when it waited for two copies in flight, the error
+ * word the attention code when it gave up, after one limit, on one that never completes. */
 TIMESTRAL_API int tsb_test_wait_expiry(int32_t kernel, int32_t* dev_error, int32_t* left_by_abort);
 /* Failure injection on the host: the next n workspace allocations of any forecast in the
  * process fail as an exhausted device would (cudaErrorMemoryAllocation); 0 clears it. */

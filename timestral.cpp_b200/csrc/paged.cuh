@@ -152,6 +152,10 @@ cudaError_t paged_attention(const PagedAttention& a, bool bf16, cudaStream_t str
 cudaError_t paged_attention_tiles(const PagedAttention& a, const PagedGrid& grid, bool bf16, cudaStream_t stream);
 constexpr int kPagedTileRows = 256;     // its rows per block
 
+// Test of drain (no fault): err[1] = 1 when it waited for two copies in flight, err[0] = kDevTimeoutAttn when it gave
+// up, after one limit, on a phase whose bytes never come all. src: 1 KB of zeros.
+cudaError_t paged_drain_selftest(int* err, const void* src, cudaStream_t stream);
+
 // A tensor map over one of the cache's pools: 64 values by up to box_slots slots of one head and
 // page, and which coordinate (1, 2 or 3) stands for what, its axes being in order of stride.
 struct PageMap {
@@ -174,6 +178,20 @@ __device__ __forceinline__ void load_page(void* dst, const PageMap& m, uint64_t*
     const int c2 = m.slot == 2 ? slot : m.head == 2 ? head : page;
     const int c3 = m.slot == 3 ? slot : m.head == 3 ? head : page;
     tma_load_4d(dst, &m.map, bar, x, c1, c2, c3);
+}
+
+// What a block still has in flight when one of its waits ran out lands before the block leaves its shared memory
+// (and tensor memory): the `count` phases of a ring of `stages` barriers from (stage, phase) on are complete,
+// or, false, one wait limit for all of them is over.
+__device__ __forceinline__ bool drain(uint64_t* bars, int stages, int stage, uint32_t phase, int count) {
+    const long long start = clock64();
+#pragma unroll 1
+    for (int i = 0; i < count; ++i) {
+        while (!mbar_try_wait(&bars[stage], phase))
+            if (clock64() - start > kWaitCycles) return false;
+        if (++stage == stages) { stage = 0; phase ^= 1; }
+    }
+    return true;
 }
 
 // The new tokens of sequence s, checked against the bounds the host gave; a contradiction is

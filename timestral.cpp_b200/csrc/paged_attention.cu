@@ -263,14 +263,18 @@ __global__ void __launch_bounds__(PR_THREADS, HD == 128 ? 1 : NR == 1 ? 5 : RG =
     for (int n = 0; n < NR; ++n) { mx[n][0] = mx[n][1] = -INFINITY; sum[n][0] = sum[n][1] = 0.f; }
 
     int st = 0, phase = 0;
-    bool expired = false;       // after an expired wait the team goes on, without waits, to meet its barriers
+    bool expired = false;       // after an expired wait the warp goes on, without waits or loads, to meet its team's barriers
     for (int tile = first; tile < last; tile += STEP) {
         const int k0 = ONE ? 0 : tile * KT;
         uint32_t valid[NW];
         bool whole = true;                          // every bit is set
 #pragma unroll
         for (int w = 0; w < NW; ++w) valid[w] = a.key_valid ? valid_word(a, t.seq, k0 + w * 32) : ~0u;
-        if (!expired && !mbar_wait(&full[st], phase)) { record_error(a.err, kDevTimeoutAttn); expired = true; }
+        if (!expired && __builtin_expect(!__all_sync(0xffffffffu, mbar_wait(&full[st], phase)), 0)) {
+            record_error(a.err, kDevTimeoutAttn);
+            expired = true;
+            if (rg == 0) drain(full, L::STAGES, st, phase, min(ONE ? 1 : L::STAGES - 1, (last - tile + STEP - 1) / STEP));
+        }
         uint8_t* const tk = ring + st * 2 * tile_bytes;
 #pragma unroll
         for (int w = 0; w < NW; ++w) whole = whole && valid[w] == ~0u;
@@ -291,7 +295,7 @@ __global__ void __launch_bounds__(PR_THREADS, HD == 128 ? 1 : NR == 1 ? 5 : RG =
         team_sync<RG>(team);                        // zeros are written; the stage read last is free
         if constexpr (!ONE) {
             const int nx = tile + (L::STAGES - 1) * STEP, ns = st == 0 ? L::STAGES - 1 : st - 1;
-            if (nx < last) load_tile(nx, ns, page);
+            if (nx < last && !expired) load_tile(nx, ns, page);
             page = page_of(nx + STEP);
         }
         const uint32_t sk = smem_u32(tk), sv = sk + tile_bytes;
@@ -558,6 +562,39 @@ __global__ void __launch_bounds__(PR_THREADS, HD == 128 ? 1 : NR == 1 ? 5 : RG =
     }
 }
 
+__global__ void drain_selftest_kernel(int* err, const uint8_t* src) {
+    __shared__ __align__(128) uint8_t buf[2][1024];
+    __shared__ uint64_t bars[2];
+    for (int i = threadIdx.x; i < 2 * 1024; i += 32) buf[i / 1024][i % 1024] = 0xff;
+    if (threadIdx.x == 0) {
+        mbar_init(&bars[0], 1);
+        mbar_init(&bars[1], 1);
+        mbar_fence_init();
+        fence_proxy_async();
+    }
+    __syncwarp();
+    auto load = [&](int s, uint32_t expected) {
+        mbar_arrive_expect_tx(&bars[s], expected);
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(buf[s])),
+                     "l"(src), "r"(1024u), "r"(smem_u32(&bars[s])) : "memory");
+    };
+    if (threadIdx.x == 0) {
+        load(1, 1024);                     // a ring of two, from its second stage on
+        load(0, 1024);
+    }
+    __syncwarp();
+    bool ok = drain(bars, 2, 1, 0, 1) && drain(bars, 2, 0, 0, 1);
+    for (int i = threadIdx.x; i < 2 * 1024; i += 32) ok = ok && buf[i / 1024][i % 1024] == 0;
+    ok = __all_sync(0xffffffffu, ok);
+    if (threadIdx.x == 0) {
+        if (ok) err[1] = 1;
+        load(1, 2 * 1024);                 // (of which the second half never comes)
+        load(0, 1024);
+    }
+    __syncwarp();
+    if (!__all_sync(0xffffffffu, drain(bars, 2, 1, 1, 2))) record_error(err, kDevTimeoutAttn);
+}
+
 // Join the splits of a row: HD / 8 threads hold a partial row, G groups of them share the splits out
 // (8 for many splits of few rows, else 2), joined through shared memory.
 template <class T, int HD, int G>
@@ -723,6 +760,11 @@ int cluster_blocks(int n, int dev, int sms) {
 }
 
 }  // namespace
+
+cudaError_t paged_drain_selftest(int* err, const void* src, cudaStream_t stream) {
+    drain_selftest_kernel<<<1, 32, 0, stream>>>(err, static_cast<const uint8_t*>(src));
+    return cudaGetLastError();
+}
 
 // A tensor map over one of the pools, its axes in order of stride (an axis of one entry has none of
 // its own).

@@ -42,7 +42,7 @@ struct TilesLayout {
 };
 
 struct TilesBars {
-    uint64_t full[8], empty[8], q_ready[2], s_full[2], p_ready[2][2], o_full[2];
+    uint64_t full[8], empty[8], q_ready[2], s_full[2], p_ready[2][2], o_full[2], done;
     uint32_t tmem;
     int abort;
 };
@@ -172,6 +172,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             mbar_init(&bars->q_ready[i], 4); mbar_init(&bars->s_full[i], 1);
             mbar_init(&bars->p_ready[i][0], 4); mbar_init(&bars->p_ready[i][1], 4); mbar_init(&bars->o_full[i], 1);
         }
+        mbar_init(&bars->done, 1);
         bars->abort = 0;
         mbar_fence_init();
         fence_proxy_async();
@@ -198,7 +199,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                 return a.cache.num_pages;                              // outside the map: zeros
             };
             int next = page_of(0), page = -1;
-            for (int i = 0; i < 2 * nt; ++i) {
+            int i = 0;
+            for (; i < 2 * nt; ++i) {
                 const int j = i >> 1, s = i % L::STAGES;
                 if ((i & 1) == 0) { page = next; next = page_of(j + 1); }
                 if (i >= L::STAGES && !role_wait_warp(&bars->empty[s], ((i / L::STAGES) - 1) & 1, abort, a.err)) break;
@@ -214,6 +216,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                 }
                 __syncwarp();
             }
+            // every load has landed before the block ends, also where an abort ends it
+            const int from = max(0, i - L::STAGES);
+            if (lane == 0) drain(bars->full, L::STAGES, from % L::STAGES, (from / L::STAGES) & 1, i - from);
+            __syncwarp();
         } else if (warp == 8) {
             {
                 // Few instructions between the MMAs, which they would hold up: descriptors differ from the ring
@@ -274,6 +280,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                     if (ok && j + 1 < nt) { mma_commit_warp(&bars->empty[slot]); next(); }
                 }
             }
+            // no MMA or commit is left when the block ends and its tensor memory is freed
+            mma_commit_warp(&bars->done);
+            if (lane == 0) drain(&bars->done, 1, 0, 0, 1);
             __syncwarp();
         }
     } else {

@@ -4,6 +4,7 @@
 #include "attention.cuh"
 #include "engine.cuh"
 #include "gemm_tc.cuh"
+#include "paged.cuh"
 #include "rows.cuh"
 #include "timestral_b200.h"
 
@@ -233,11 +234,12 @@ extern "C" TIMESTRAL_API int tsb_test_refine(const float* d_q, const float* d_ro
 
 extern "C" TIMESTRAL_API int tsb_test_wait_expiry(int32_t kernel, int32_t* dev_error, int32_t* left_by_abort) {
     using namespace tsb;
-    if (kernel != 0 && kernel != 1) return TSB_ERR_ARG;
-    int* d = nullptr;
-    if (cudaMalloc(&d, 2 * sizeof(int)) != cudaSuccess) return TSB_ERR_CUDA;
-    cudaError_t ce = cudaMemset(d, 0, 2 * sizeof(int));
-    if (ce == cudaSuccess) ce = kernel == 0 ? gemm_wait_expiry_selftest(d, 0) : attention_wait_expiry_selftest(d, 0);
+    if (kernel < 0 || kernel > 2) return TSB_ERR_ARG;
+    int* d = nullptr;                                      // the two words; 1 KB of zeros behind them (kernel 2)
+    if (cudaMalloc(&d, 2048) != cudaSuccess) return TSB_ERR_CUDA;
+    cudaError_t ce = cudaMemset(d, 0, 2048);
+    if (ce == cudaSuccess)
+        ce = kernel == 0 ? gemm_wait_expiry_selftest(d, 0) : kernel == 1 ? attention_wait_expiry_selftest(d, 0) : paged_drain_selftest(d, d + 256, 0);
     if (ce == cudaSuccess) ce = cudaDeviceSynchronize();
     int h[2] = {0, 0};
     if (ce == cudaSuccess) ce = cudaMemcpy(h, d, sizeof(h), cudaMemcpyDeviceToHost);

@@ -229,6 +229,12 @@ struct Engine::Impl {
         int width = 0;           // pages of a row
         int sublayer = 0;        // time sublayers run so far in the current block
         DevBuf kv, table, q_start, lengths, feat, rope, workspace;
+        bool release() {         // false: it held nothing
+            on = false;
+            if (!kv.p && !workspace.p) return false;
+            for (DevBuf* b : {&kv, &table, &q_start, &lengths, &feat, &rope, &workspace}) b->release();
+            return true;
+        }
     } cache;
     int time_sublayers() const {
         int n = 0;
@@ -1386,10 +1392,10 @@ void Engine::decoder_tail(bool on) {
 
 void Engine::decode_cache(bool on) {
     Impl& im = *impl_;
-    if (!on && im.cache.kv.p) {
+    if (!on) {
         check(cudaSetDevice(device_), "cudaSetDevice");
         check(cudaStreamSynchronize(stream_), "sync");
-        im.cache.kv.release();
+        im.cache.release();
     }
     im.cache.enabled = on;
 }

@@ -103,7 +103,9 @@ TIMESTRAL_API int tsb_decoder_tail(timestral_ctx* ctx, int32_t on);
  * forecast stays within the f16 path's deviation but is not the same bits: the attention over the
  * cache sums in another order. A forecast whose context slides past max_context, one of several
  * rows per series, tsb_attention_kernels mode 1, and one whose cache would take more than half of
- * the free device memory run as with on = 0. */
+ * the free device memory (what the cache holds already counted as free) or for which the memory
+ * runs out run as with on = 0. The cache's memory is kept for the next forecast; another that
+ * finds none takes it, and on = 0 gives back all of it. */
 TIMESTRAL_API int tsb_decode_cache(timestral_ctx* ctx, int32_t on);
 /* CUDA-graph replay (on by default): a forecast without covariates that fits one decode
  * block (H <= 32 patches of the 209M geometry) is captured into a CUDA graph on its second

@@ -20,6 +20,7 @@
 #include <cmath>
 #include <cstdio>
 #include <cstring>
+#include <functional>
 #include <memory>
 #include <stdexcept>
 
@@ -77,6 +78,13 @@ bool take_injected_failure() {
     return false;
 }
 
+// A workspace allocation found no memory.
+struct OutOfMemory : std::runtime_error {
+    using std::runtime_error::runtime_error;
+};
+// While an engine's call runs on this thread: gives back memory that the call can do without (false: there is none).
+thread_local const std::function<bool()>* g_spare_memory = nullptr;
+
 struct DevBuf {
     void* p = nullptr;
     size_t bytes = 0;
@@ -88,9 +96,16 @@ struct DevBuf {
         if (n <= bytes) return;
         g_workspace_generation.fetch_add(1);
         if (p) { cudaFree(p); p = nullptr; bytes = 0; }
-        check(take_injected_failure() ? cudaErrorMemoryAllocation : cudaMalloc(&p, std::max<size_t>(n, 256)),
-              "cudaMalloc workspace");
+        cudaError_t e = allocate(n);
+        if (e == cudaErrorMemoryAllocation && g_spare_memory && (*g_spare_memory)()) e = allocate(n);
+        if (e == cudaErrorMemoryAllocation) throw OutOfMemory(std::string("cudaMalloc workspace: ") + cudaGetErrorString(e));
+        check(e, "cudaMalloc workspace");
         bytes = std::max<size_t>(n, 256);
+    }
+    cudaError_t allocate(size_t n) {
+        const cudaError_t e = take_injected_failure() ? cudaErrorMemoryAllocation : cudaMalloc(&p, std::max<size_t>(n, 256));
+        if (e != cudaSuccess) { p = nullptr; cudaGetLastError(); }     // (not to be found by the next launch's check)
+        return e;
     }
     void release() {
         if (!p) return;
@@ -236,6 +251,16 @@ struct Engine::Impl {
             return true;
         }
     } cache;
+    // Memory that the cache holds and the running forecast does not use is free for its other buffers.
+    const std::function<bool()> spare_cache = [this] { return !cache.on && cache.release(); };
+    struct SparesCache {
+        const std::function<bool()>* before = g_spare_memory;
+        explicit SparesCache(Impl& im) {
+            im.cache.on = false;                             // (of the forecast before)
+            g_spare_memory = &im.spare_cache;
+        }
+        ~SparesCache() { g_spare_memory = before; }
+    };
     int time_sublayers() const {
         int n = 0;
         for (const auto& layer : attn)
@@ -252,14 +277,21 @@ struct Engine::Impl {
         if (need > cache.kv.bytes) {
             size_t free_bytes = 0, total = 0;
             check(cudaMemGetInfo(&free_bytes, &total), "cudaMemGetInfo");
-            if (need > free_bytes / 2) return;               // the blocks run their whole context again
+            if (need > (free_bytes + cache.kv.bytes) / 2) return;        // the blocks run their whole context again
         }
-        cache.kv.ensure(need);
         cache.width = width;
-        cache.table.ensure(size_t(R2) * width * 4);
-        cache.q_start.ensure(size_t(R2 + 1) * 4);
-        cache.lengths.ensure(size_t(R2) * 4);
-        cache.on = true;
+        cache.on = true;                                     // from here on its buffers are not to spare
+        try {
+            cache.kv.ensure(need);
+            cache.table.ensure(size_t(R2) * width * 4);
+            cache.q_start.ensure(size_t(R2 + 1) * 4);
+            cache.lengths.ensure(size_t(R2) * 4);
+            // of a later block: its new patches' features, its row's positions
+            cache.feat.ensure(size_t(R2) * h * 2 * ps * 4);
+            cache.rope.ensure(size_t(R2) * (context + h) * 4);
+        } catch (const OutOfMemory&) {
+            cache.release();
+        }
     }
     // The time sublayer's attention over the cache: q, k, v, gate token-major [R2 * S][H][64].
     void cached_attention(int R2, int S, const MaskMeta& mm, const __half* gate, __half* out) {
@@ -1254,7 +1286,7 @@ void Engine::forecast_targets(const float* d_ctx, const uint8_t* d_umask, int B,
         check(cudaStreamBeginCapture(s, cudaStreamCaptureModeThreadLocal), "begin capture");
     }
     try {
-        targets_body(d_ctx, d_umask, B, V, T, H, symmetric, clip, d_out, kept, len, patches, shot, R, R2, cap);
+        targets(d_ctx, d_umask, B, V, T, H, symmetric, clip, d_out, kept, len, patches, shot, R, R2, cap);
     } catch (...) {
         if (capture) {
             cudaGraph_t g = nullptr;
@@ -1294,8 +1326,8 @@ void Engine::finish_targets() {
     const Impl::Pending p = im.pending;
     im.fuse_now = false;
     try {
-        targets_body(static_cast<const float*>(p.ctx), static_cast<const uint8_t*>(p.umask), p.B, p.V, p.T, p.H, p.sym,
-                     p.clip, static_cast<float*>(p.out), p.kept, p.len, p.patches, p.shot, p.R, p.R2, p.cap);
+        targets(static_cast<const float*>(p.ctx), static_cast<const uint8_t*>(p.umask), p.B, p.V, p.T, p.H, p.sym,
+                p.clip, static_cast<float*>(p.out), p.kept, p.len, p.patches, p.shot, p.R, p.R2, p.cap);
     } catch (...) {
         im.fuse_now = true;
         throw;
@@ -1304,8 +1336,31 @@ void Engine::finish_targets() {
     im.check_device_error("forecast");
 }
 
+void Engine::targets(const float* d_ctx, const uint8_t* d_umask, int B, int V, int T, int H, bool symmetric,
+                     bool clip, float* d_out, int kept, int len, int patches, int shot, int R, int R2, int cap) {
+    Impl& im = *impl_;
+    const Impl::SparesCache spares(im);
+    const auto launches = im.launches;
+    const size_t events = im.ev_used;
+    auto body = [&](bool cached) {
+        targets_body(d_ctx, d_umask, B, V, T, H, symmetric, clip, d_out, kept, len, patches, shot, R, R2, cap, cached);
+    };
+    try {
+        body(true);
+        return;
+    } catch (const OutOfMemory&) {
+        if (!im.cache.on) throw;
+    }
+    // What the decode cache holds is missing elsewhere: once more from the start, without it.
+    check(cudaStreamSynchronize(stream_), "forecast");
+    im.cache.release();
+    im.launches = launches;
+    im.ev_used = events;
+    body(false);
+}
+
 void Engine::targets_body(const float* d_ctx, const uint8_t* d_umask, int B, int V, int T, int H, bool symmetric,
-                          bool clip, float* d_out, int kept, int len, int patches, int shot, int R, int R2, int cap) {
+                          bool clip, float* d_out, int kept, int len, int patches, int shot, int R, int R2, int cap, bool cached) {
     Impl& im = *impl_;
     const ModelView& mv = im.mv;
     const int ps = im.ps, Q = im.Q;
@@ -1325,7 +1380,7 @@ void Engine::targets_body(const float* d_ctx, const uint8_t* d_umask, int B, int
     // one, and with it other positions, from the fed back medians; its older patches stay unseen.)
     const int longest = len + (patches - 1) / shot * shot * ps;
     im.cache.on = false;
-    if (im.cache.enabled && !single && im.tc && im.hd == 64 && V == 1 && !im.attn_simt && longest <= cap)
+    if (cached && im.cache.enabled && !single && im.tc && im.hd == 64 && V == 1 && !im.attn_simt && longest <= cap)
         im.start_cache(R2, longest / ps, shot);
     (void)T;
     while (done < patches) {
@@ -1419,6 +1474,7 @@ void Engine::decode_host_rows(const HostRows& a, int H, float* h_decoded) {
     Range range("tsb decode");
     check(cudaSetDevice(device_), "cudaSetDevice");
     Impl& im = *impl_;
+    const Impl::SparesCache spares(im);
     if (im.pending.valid && im.fuse_now) {       // an earlier asynchronous forecast: complete it
         check(cudaStreamSynchronize(stream_), "forecast");
         finish_targets();
@@ -1460,6 +1516,7 @@ void Engine::forecast_rows(const HostRows& a, int B, int V, int H, bool symmetri
     Range range("tsb forecast (host rows)");
     check(cudaSetDevice(device_), "cudaSetDevice");
     Impl& im = *impl_;
+    const Impl::SparesCache spares(im);
     if (im.pending.valid && im.fuse_now) {       // an earlier asynchronous forecast: complete it
         check(cudaStreamSynchronize(stream_), "forecast");
         finish_targets();
@@ -1526,6 +1583,7 @@ void Engine::forecast_covariates(const CovRequest& q, bool symmetric, bool clip,
     Range range("tsb forecast (covariates)");
     check(cudaSetDevice(device_), "cudaSetDevice");
     Impl& im = *impl_;
+    const Impl::SparesCache spares(im);
     if (im.pending.valid && im.fuse_now) {       // an earlier asynchronous forecast: complete it
         check(cudaStreamSynchronize(stream_), "forecast");
         finish_targets();

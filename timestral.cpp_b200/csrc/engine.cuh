@@ -176,8 +176,11 @@ public:
 
 private:
     void finish_targets();
+    // A forecast's work: targets_body, and where the decode cache leaves it without memory once more without the cache.
+    void targets(const float* d_ctx, const uint8_t* d_umask, int B, int V, int T, int H, bool symmetric, bool clip,
+                 float* d_out, int kept, int len, int patches, int shot, int R, int R2, int cap);
     void targets_body(const float* d_ctx, const uint8_t* d_umask, int B, int V, int T, int H, bool symmetric, bool clip,
-                      float* d_out, int kept, int len, int patches, int shot, int R, int R2, int cap);
+                      float* d_out, int kept, int len, int patches, int shot, int R, int R2, int cap, bool cached);
     // The decode blocks of an assembled covariate request (rows, masks, roles, futures in
     // device memory) through the final download.
     void decode_rows(int B, int V, int H, int R, int T, int Hh, bool symmetric, bool clip, bool cov, bool has_future,

@@ -708,7 +708,6 @@ template <class T, int HD, int G>
 cudaError_t launch_combine(const PagedAttention& a, const PagedGrid& grid, int tile_rows, cudaStream_t stream) {
     constexpr int ROWS = 128 / (HD / 8 * G);
     const int64_t rows = int64_t(grid.items - grid.whole) * tile_rows;
-    if (rows > INT32_MAX - ROWS) return cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned((rows + ROWS - 1) / ROWS));
     cfg.blockDim = dim3(128);
@@ -914,7 +913,8 @@ void paged_workspace(PagedAttention* a, void* workspace, size_t bytes) {
 cudaError_t paged_attention(const PagedAttention& a, bool bf16, cudaStream_t stream) {
     const PagedPlan p = paged_plan(a);
     const int64_t whole = a.splits > 1 ? p.whole : p.items, units = whole + (p.items - whole) * a.splits;
-    if (units > INT32_MAX - 4) return cudaErrorInvalidValue;
+    // (asked before the first kernel is on the stream, which the join's grid would be too late for)
+    if (units > INT32_MAX - 4 || (a.part_o && (p.items - whole) * p.tile_rows > INT32_MAX - 128)) return cudaErrorInvalidValue;
     PagedGrid g;
     g.splits = FastDiv(uint32_t(a.splits));
     g.heads = FastDiv(uint32_t(a.cache.kv_heads));

@@ -4,6 +4,7 @@
                     [--batch B] [--no-cpu] [--no-e2e]
     python bench.py --impl reference ...   # the CPU reference arm (rank 0 only)
     python bench.py --compare-cublas       # the fused GEMMs against cuBLAS at the cfg5 shapes
+    python bench.py --compare-decode-cache # forecasts of several decode blocks with the decode cache off and on
 
 Workloads (209M architecture, random init seed 0, synthetic series of each config's shape;
 symmetric averaging and clipping on):
@@ -112,6 +113,8 @@ def parse():
     ap.add_argument("--no-cpu", action="store_true")
     ap.add_argument("--compare-cublas", action="store_true",
                     help="time each fused GEMM kind and cuBLAS (torch.mm, f16 in/out) at the cfg5 token count")
+    ap.add_argument("--compare-decode-cache", action="store_true",
+                    help="time forecasts of several decode blocks with the decode cache off and on (209M f16)")
     a = ap.parse_args()
     c = dict(CONFIGS[a.config])
     c.setdefault("cpu_sample_1t", 1)
@@ -420,10 +423,50 @@ def compare_cublas(seconds: float = 2.0):
     return 0
 
 
+def compare_decode_cache(steps: int = 5, warmup: int = 3, rounds: int = 3):
+    """Forecasts of several decode blocks (209M f16 random-init, both passes and clipping, context in device
+    memory, other random walks at each size) with the decode cache off and on in turn: the median
+    over `rounds` of CUDA-event times of `steps` forecasts each; one JSON line per size. From 64 series on
+    a forecast's working set is far above the 126 MB L2."""
+    import torch
+    import timestral_b200 as tb
+    from timestral_b200 import synthetic as sy
+    dev = torch.device("cuda:0")
+    torch.cuda.set_device(dev)
+    model = tb.Model(sy.cached_model(sy.spec_209m(), "f16"))
+    stream = torch.cuda.ExternalStream(model.stream(), device=dev)
+    for B, T, H in ((1, 2048, 4096), (64, 2048, 4096), (512, 2048, 4096), (64, 8192, 8192)):
+        d_ctx = torch.from_numpy(sy.series_random_walk(B, T, nan_frac=0.05)).to(dev)
+        d_out = torch.empty((B, 1, H, model.num_quantiles), device=dev)
+        torch.cuda.synchronize()
+        times = {False: [], True: []}
+        clk = ClockSampler(0)
+        clk.start()
+        for _ in range(rounds):
+            for on in (False, True):
+                model.decode_cache(on)
+                e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+                for i in range(warmup + steps):
+                    if i == warmup:
+                        e0.record(stream)
+                    model.forecast_device(d_ctx.data_ptr(), None, B, 1, T, H, d_out.data_ptr(), asynchronous=True)
+                e1.record(stream)
+                e1.synchronize()
+                if tb.lib().tsb_sync(model.h) != 0:
+                    raise RuntimeError(model.last_error)
+                times[on].append(e0.elapsed_time(e1) / steps)
+        off, on = (float(np.median(times[k])) for k in (False, True))
+        print(json.dumps({"forecast": f"209M f16, B={B} V=1 T={T} H={H}", "ms_cache_off": round(off, 2), "ms_cache_on": round(on, 2),
+                          "ratio": round(off / on, 2), "steps": steps, "warmup": warmup, "rounds": rounds, "clocks": clk.stop()}), flush=True)
+    return 0
+
+
 def main():
     a, c = parse()
     if a.compare_cublas:
         return compare_cublas()
+    if a.compare_decode_cache:
+        return compare_decode_cache()
     rank = int(os.environ.get("RANK", "0"))
     world = int(os.environ.get("WORLD_SIZE", "1"))
     local = int(os.environ.get("LOCAL_RANK", "0"))

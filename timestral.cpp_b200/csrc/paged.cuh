@@ -127,7 +127,7 @@ __device__ __forceinline__ uint32_t unit_of(const PagedGrid& g, uint32_t unit, u
 // How a call of paged_attention runs: chosen from sizes alone, so that the workspace query and
 // the call agree. splits is what it would like without a bound on the workspace.
 struct PagedPlan {
-    bool tiles = false;                 // paged_attention_tiles, else paged_attention_rows
+    bool tiles = false;                 // paged_tiles_kernel, else paged_rows_kernel
     bool join = false;                  // rows: a block's teams share one problem
     bool one = false;                   // rows: a tile holds every key
     int tile_rows = 0;

@@ -184,7 +184,9 @@ TIMESTRAL_API int tsb_refine_static(const float* d_q, const float* d_rows, const
  * Common rules. Every pointer is memory of the current device (anything else is refused with
  * TSB_ERR_ARG), as is `stream` (cudaStream_t, NULL = legacy default stream). Calls enqueue
  * work and return; they allocate nothing, keep nothing between calls and may be captured into
- * a CUDA graph. Values are f16 or bf16, sums and statistics f32, each result is rounded once.
+ * a CUDA graph. Values are f16 or bf16, sums and statistics f32, each result is rounded once;
+ * tsb_paged_attention also rounds each key's probability to the type of the values before it
+ * weighs them (at most half a step of that type, relative to the weighted mean of |v|).
  * The last axis (head_dim) is contiguous; every pointer to values, weights or angles is 16-byte
  * aligned and every stride of values, in elements, a multiple of 8. Offsets are 64-bit. Argument errors go to
  * timestral_capi_last_error(NULL).

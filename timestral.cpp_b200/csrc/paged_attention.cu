@@ -2,7 +2,9 @@
 // window, key-valid bits, optional gate.
 //
 // out = gate * sum_j p_j v_j / sum_j p_j with p_j = 2^(t_j - m), t_j = (q . k_j) * scale * log2(e),
-// m a running maximum: one pass over the keys that keeps m, the sum and the weighted values in f32.
+// m a running maximum: one pass over the keys that keeps m, the sum and the weighted values in f32. The p_j are
+// rounded to the values' type for the second product, whose MMA takes 16-bit operands (their sum is taken before):
+// at most half a step of that type relative to each, so of the weighted mean of |v|.
 // The rows of one (sequence, cached head) problem are its (token, query head of the group) pairs,
 // row = token * group + head, so that a cached key is read once for the whole group.
 #include "paged.cuh"
@@ -787,14 +789,17 @@ bool page_maps(PageMaps* m, const PagedCache& c, bool bf16, int box_slots) {
            page_map(&m->v, c.v, bf16, c, c.v_page, c.v_head, c.v_slot, box_slots);
 }
 
-// Which way to run a call: an estimate in microseconds of each, and the least is taken. It goes by sizes
-// alone (the bounds that the host knows; the lengths stand on the device). Rounds of units (a problem's
-// keys or a share of them), each with a start and its keys, where a unit goes at the rate of its own
-// teams' loads or at its part of what an SM loads, whichever is slower. The constants below were fitted
-// to the best choice over 9,983 calls (1 to 256 rows, 97 to 198,000 keys, 1 to 512 sequences, 2 to 16
-// cached heads, even and uneven lengths), each timed in every way open to it: on average the chosen way
-// took 1.02 times the best one's time, 1.13 at the 95th percentile, 1.42 at worst. Fixed bounds on rows
-// and keys (teams joined above 256 keys, tiles above 64 rows) took 1.16, 1.75 and 5.6.
+// Which way to run a call: a figure for each, and the least is taken. It goes by sizes alone (the bounds that the
+// host knows; the lengths stand on the device): rounds of units (a problem's keys or a share of them), each with a
+// start and its keys, where a unit goes at the rate of its own teams' loads or at its part of what an SM loads,
+// whichever is slower. The figures rank the ways and are near microseconds, but are no prediction: the constants
+// were fitted to the best choice over even and uneven lengths together, which sets them below what even lengths
+// take (kShared of head_dim 128 is twice the memory's rate), and pages count as whole tiles (pages of 64, 16 and
+// 8 positions take a decode batch of 64 sequences, 8,192 keys and 8 cached heads of 128 318, 336 and 379 us: a load
+// for each page). Fitted to 9,983 calls (1 to 256 rows, 97 to 198,000 keys, 1 to 512 sequences, 2 to 16 cached
+// heads, even and uneven lengths), each timed in every way open to it by a build that forces the way: the
+// chosen way took 1.02 times the best one's time on average, 1.13 at the 95th percentile, 1.42 at worst; fixed
+// bounds on rows and keys (teams joined above 256 keys, tiles above 64 rows) 1.16, 1.75 and 5.6.
 // Both sides, us: one row over 500 keys of 64, 24,576 problems: a team each 520, teams joined 604, and
 // over 800 keys, 96 problems: 33 and 16; 64 rows over 4,016 keys of 128, 512 problems: rows 303, tiles 242,
 // and over 128 keys of 64, 12,288 problems: rows 213, tiles 555; 16 problems over 11,000 keys of 128, clusters

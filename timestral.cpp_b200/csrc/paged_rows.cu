@@ -1,9 +1,9 @@
 // Per-head norm and rotation of queries and keys (norm_rope), and writing keys and values into
 // a paged cache with the same norm and rotation on the way (paged_append).
 //
-// Both read every value once and write it once: the memory rate bounds them (68.5 us and 0.77
-// of the copy rate for norm and rotation of 16,384 tokens of 40 heads of 128; 24.6 us, 0.80, for 64 uneven prompts
-// of up to 512 tokens appended; 38.7 us, 0.79, for 32,768 tokens of 12 heads of 64 appended as they are). A head is held by
+// Both read every value once and write it once: the memory rate bounds them (other buffers each time: 66 to 68 us and
+// 0.78 of the copy rate for norm and rotation of 16,384 tokens of 40 heads of 128; 24.7 us, 0.80, for 64 uneven prompts
+// of up to 512 tokens appended; 38.6 us, 0.79, for 32,768 tokens of 12 heads of 64 appended as they are). A head is held by
 // PT threads (head_dim / 16, rounded up to a power of two), each with two vectors of eight values
 // whose elements the rotation pairs (d and d + rope_dim / 2; behind rope_dim two neighbouring
 // vectors that nothing turns), so that the rotation needs no exchange and the sum of squares is
@@ -58,7 +58,7 @@ __device__ __forceinline__ void load8(const float* p, float (&f)[8]) {
 
 // Sixteen bytes that this call reads (writes) once. HINT: first to leave L2, so that the copies which wait
 // there to be written back do not push out what is still to be read. Passes over the same buffers, norm and
-// rotation of 16,384 tokens of 40 heads of 128: 61.2 us, without the hint 64.5 (other buffers each time: 68.5, 68.9); a reader right behind it takes as long
+// rotation of 16,384 tokens of 40 heads of 128: 61.2 us, without the hint 64.5 (other buffers each time it gains less, 0.4 us); a reader right behind it takes as long
 // either way (123.3 and 123.8 with it). 64 prompts of 512 tokens appended with a rotation: 20.6 and 22.9. The
 // plain copy goes without (2,048 rows of 16 tokens: 36.4, with it 37.1).
 template <bool HINT>

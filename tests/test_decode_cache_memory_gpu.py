@@ -95,3 +95,31 @@ def test_off_gives_back_what_the_cache_held():
     assert free() < before - (16 << 20)
     m.decode_cache(False)
     assert free() >= before - (2 << 20)
+
+
+def test_nothing_stays_of_a_cache_that_found_no_memory():
+    """Its keys and values are to grow and cannot: the rest of it (8 MB here) goes too."""
+    path = sy.cached_model(sy.spec_small(), "f16")
+    x = sy.series_random_walk(512, 640)
+    m, other = tb.Model(path), tb.Model(path)
+    other.decode_cache(True)
+    other.forecast(x, 2600)
+    other.close()
+
+    def free():
+        torch.cuda.synchronize()
+        return torch.cuda.mem_get_info()[0]
+    for H in (2600, 1500, 2600):                  # (until both buffers of contexts are as large as they get)
+        off = m.forecast(x, H).copy()
+    plain, before = m.last_geometry(), free()
+    m.decode_cache(True)
+    m.forecast(x, 1500)
+    assert free() < before - (16 << 20)
+    with fail_next_allocation():
+        got = m.forecast(x, 2600).copy()
+    assert same(got, off) and m.last_geometry() == plain
+    assert free() >= before - (2 << 20)
+    m.forecast(x, 2600)
+    assert m.last_geometry() != plain
+    m.decode_cache(False)
+    assert free() >= before - (2 << 20)

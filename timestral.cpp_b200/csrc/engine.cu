@@ -244,11 +244,12 @@ struct Engine::Impl {
         int width = 0;           // pages of a row
         int sublayer = 0;        // time sublayers run so far in the current block
         DevBuf kv, table, q_start, lengths, feat, rope, workspace;
+        bool holds() const { return kv.p || table.p || q_start.p || lengths.p || feat.p || rope.p || workspace.p; }
         bool release() {         // false: it held nothing
             on = false;
-            if (!kv.p && !workspace.p) return false;
+            const bool any = holds();
             for (DevBuf* b : {&kv, &table, &q_start, &lengths, &feat, &rope, &workspace}) b->release();
-            return true;
+            return any;
         }
     } cache;
     // Memory that the cache holds and the running forecast does not use is free for its other buffers.
@@ -1447,7 +1448,7 @@ void Engine::decoder_tail(bool on) {
 
 void Engine::decode_cache(bool on) {
     Impl& im = *impl_;
-    if (!on) {
+    if (!on && im.cache.holds()) {
         check(cudaSetDevice(device_), "cudaSetDevice");
         check(cudaStreamSynchronize(stream_), "sync");
         im.cache.release();

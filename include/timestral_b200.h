@@ -200,11 +200,13 @@ enum {
     TSB_FAULT_POSITION = 6,  /* a position outside the rotation table: that token is not written */
     TSB_FAULT_BATCH = 10,    /* q_start or lengths contradict each other or the given bounds: that
                                 sequence is skipped, its rows left as they were */
-    TSB_FAULT_PAGE = 11,     /* a page number outside the pool: nothing is written there, and its
-                                keys and values read as zeros */
+    TSB_FAULT_PAGE = 11,     /* a page number outside the pool, where a position is to be written or
+                                is visible: nothing is written there, and its keys and values
+                                read as zeros */
 };
 
-/* [tokens][heads][head_dim]: element (t, h, d) at data[t * token_stride + h * head_stride + d]. */
+/* [tokens][heads][head_dim]: element (t, h, d) at data[t * token_stride + h * head_stride + d]. Heads do
+ * not overlap (a head_stride of at least head_dim, where there are several); tokens of an input may. */
 typedef struct tsb_heads {
     void* data;
     int64_t token_stride, head_stride;
